@@ -141,7 +141,9 @@ int nr_add_layernorm_bwd_noalloc_f32(const float* dy, const float* s, const floa
  * row_max/row_sum [N,H,S] (may be NULL in eval) are the softmax statistics the backward reuses.
  * mask_mode 0: masked keys get an additive -1e5 in fp32 before the softmax (attention.py:44-49,90);
  * mask_mode 1: masked keys are excluded and a sequence without any valid key gets zero probabilities — what
- *   HF BertModel computes under torch SDPA for AllBertNewsEncoder (encoder.py:74; transformers 5.15 / torch 2.10). */
+ *   HF BertModel computes under torch SDPA for AllBertNewsEncoder (encoder.py:74; transformers 5.15 / torch 2.10).
+ * Any S; head dims up to 128.  Sequences of S <= 128 run on kernels that hold a whole head at once, longer ones (and the head dims
+ * those kernels do not take) on the key-tiled kernels of nr_attention_fwd / _bwd below, which S has no bound for. */
 int nr_mhsa_fwd_f32(const float* qkv, const int64_t* mask, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* ctx, float* row_max, float* row_sum, void* stream);
 int nr_mhsa_bwd_f32(const float* qkv, const int64_t* mask, const float* ctx, const float* dctx, const float* row_max, const float* row_sum, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* dqkv, void* stream);
 /* The same core on bf16 tensors (raw 16-bit storage; S <= 32, head dim <= 64): what the bf16 build of AllBertNewsEncoder's
@@ -150,6 +152,34 @@ int nr_mhsa_bwd_f32(const float* qkv, const int64_t* mask, const float* ctx, con
  * other head dims take f32 arithmetic on the bf16 data. */
 int nr_mhsa_fwd_bf16(const void* qkv, const int64_t* mask, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, void* ctx, float* row_max, float* row_sum, void* stream);
 int nr_mhsa_bwd_bf16(const void* qkv, const int64_t* mask, const void* dctx, const float* row_max, const float* row_sum, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, void* dqkv, void* stream);
+
+/* ---- softmax attention of any length -------------------------------------------------------------------------------
+ * out[n,i,h] = sum_j p_ij v[n,j,g],  p_i = softmax over j of scale * q[n,i,h] . k[n,j,g],  g = h / (H / G)
+ * (the reference's attention core, attention.py:87-97, without its bound on the length, for queries and keys of different
+ * lengths, shared key heads and causal order).  A key j takes part if key_mask[n,j] != 0 (key_mask [N,Sk] int64, NULL: all) and,
+ * with causal, j <= i + Sk - Sq: the last query stands at the last key.  A row without any key is zero and sends no gradient.
+ * Rows of k / v whose mask is 0 are never used, whatever they hold; with causal order alone a later row of the same sequence
+ * that is not finite can reach earlier queries of its tile (as 0 * inf).
+ * q [N,Sq,H,dh], k / v [N,Sk,G,dh]: dtype 0 = fp32, 1 = bf16; innermost axis dense, the other strides in elements, any (0 as
+ * well); multiples of 16 bytes throughout run faster.  out, dout, dq, dk, dv: dense, same dtype.  dh <= 128.
+ * row_max / row_sum [N,H,Sq] fp32 (NULL in evaluation): the softmax statistics that the backward reuses.
+ * Dropout on the probabilities: element index ((n*H + h)*Sq + i)*Sk + j of (seed, site).
+ * ws: nr_attention_{fwd,bwd}_ws_bytes(p) bytes (0 for most sizes), scratch of this call alone. */
+typedef struct {
+    const void *q, *k, *v;
+    const int64_t *key_mask;
+    int64_t N, Sq, Sk, H, G, dh;
+    int64_t q_stride[3], k_stride[3], v_stride[3];      /* sequence, position, head */
+    int32_t dtype, causal;
+    float scale, p_drop;
+    uint64_t seed;
+    uint32_t site;
+} nr_attention;
+size_t nr_attention_fwd_ws_bytes(const nr_attention* p);
+int nr_attention_fwd(const nr_attention* p, void* out, float* row_max, float* row_sum, void* ws, size_t ws_bytes, void* stream);
+/* delta [N,H,Sq] fp32 is scratch of the call besides ws.  Fixed summation order: the same bits every time. */
+size_t nr_attention_bwd_ws_bytes(const nr_attention* p);
+int nr_attention_bwd(const nr_attention* p, const void* out, const void* dout, const float* row_max, const float* row_sum, float* delta, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- additive ("query") pooling — scaled_dp_attention, attention.py:6-34 -----------------------
  * out[n,:] = softmax_s(query . key[n,s,:] / sqrt(D) + (1-mask[n,s]) * -1e5) . value[n,s,:]

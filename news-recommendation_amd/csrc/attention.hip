@@ -1,4 +1,5 @@
-// Multi-head self-attention over short sequences (titles S=32, histories S=50, title+abstract S=96; S <= 128),
+// Multi-head self-attention over short sequences (titles S=32, histories S=50, title+abstract S=96; S <= 128; longer ones are
+// handed to attention_long.hip),
 // one wave (two for S > 64) per (sequence, head).  The S x S score tile is tiny (<= 16 KiB), so the whole
 // head lives in LDS/registers: lane i owns query row i (fwd, bwd phase A) or key row j
 // (bwd phase B).  Score arithmetic follows the reference literally:
@@ -8,6 +9,8 @@
 // ~1-2 % of the layer's flops: plain VALU fma (the f32 MFMA rate equals the f32 VALU rate).
 #include "common.h"
 #include "seqops.h"
+#include "attention_long.h"
+#include <math.h>
 
 namespace nr {
 
@@ -338,6 +341,40 @@ __global__ __launch_bounds__(NT) void mhsa_bwd_recompute_kernel(const float* __r
 constexpr size_t MHSA_LDS_MAX = 160 * 1024;    // one workgroup may take the CU's whole LDS
 static int pick_dhp(int dh) { return dh <= 32 ? 32 : (dh <= 64 ? 64 : (dh <= 128 ? 128 : 0)); }
 
+// sequences past 128 positions, and head dims past what the kernels above hold in LDS: the key-tiled kernels of
+// attention_long*.hip on the q | k | v blocks of the packed rows, with this layer's additive mask
+static AttnProblem long_problem(const float* qkv, const int64_t* mask, int64_t N, int S, int H, int dh, const DropoutCfg& dc) {
+    AttnProblem p;
+    const int64_t A = (int64_t)H * dh;
+    p.q = qkv; p.k = qkv + A; p.v = qkv + 2 * A; p.key_mask = mask;
+    p.sq = p.sk = p.sv = AttnStrides{(int64_t)S * 3 * A, 3 * A, dh};
+    p.N = N; p.Sq = p.Sk = S; p.H = p.G = H; p.dh = dh;
+    p.additive = dc.mask_fill != -INFINITY;
+    p.scale = (float)(1.0 / sqrt((double)dh));
+    p.dc = dc;
+    return p;
+}
+static int mhsa_long_fwd(const float* qkv, const int64_t* mask, float* ctx, float* row_max, float* row_sum, int64_t N, int S, int H, int dh,
+                         const DropoutCfg& dc, hipStream_t s) {
+    const int64_t A = (int64_t)H * dh;
+    AttnOut o;
+    o.out = ctx; o.so = AttnStrides{S * A, A, dh}; o.row_max = row_max; o.row_sum = row_sum;
+    ProfScope prof(FAM_ATTN, s, 4.0 * N * H * S * S * dh);
+    return attn_long_fwd(long_problem(qkv, mask, N, S, H, dh, dc), o, nullptr, 0, s);
+}
+static int mhsa_long_bwd(const float* qkv, const int64_t* mask, const float* ctx, const float* dctx, const float* row_max, const float* row_sum,
+                         float* dqkv, int64_t N, int S, int H, int dh, const DropoutCfg& dc, hipStream_t s) {
+    const int64_t A = (int64_t)H * dh;
+    AttnGrad g;
+    g.out = ctx; g.dout = dctx; g.so = g.sdo = AttnStrides{S * A, A, dh};
+    g.row_max = row_max; g.row_sum = row_sum;
+    g.dq = dqkv; g.dk = dqkv + A; g.dv = dqkv + 2 * A;
+    g.sdq = g.sdk = g.sdv = g.sd = AttnStrides{(int64_t)S * 3 * A, 3 * A, dh};
+    g.delta = dqkv;                              // the first element of each row's dq, written last (attention_long.h)
+    ProfScope prof(FAM_ATTN, s, 10.0 * N * H * S * S * dh);
+    return attn_long_bwd(long_problem(qkv, mask, N, S, H, dh, dc), g, nullptr, 0, s);
+}
+
 int mhsa_fwd(const float* qkv, const int64_t* mask, float* ctx, float* row_max, float* row_sum, int64_t N, int S, int H,
              int dh, DropoutCfg dc, hipStream_t s) {
     if (N == 0) return NR_OK;
@@ -350,11 +387,11 @@ int mhsa_fwd(const float* qkv, const int64_t* mask, float* ctx, float* row_max, 
         return mhsa_fwd_mfma2(qkv, mask, ctx, row_max, row_sum, N, S, H, dh, dc, s);
     }
     NR_UNSUPPORTED(dc.offs != nullptr, "mhsa: packed sequences need S <= 64 and head dim <= 64 (got S=%d, dh=%d)", S, dh);
-    NR_UNSUPPORTED(S > 128 || S < 1, "mhsa: sequence length %d not in [1,128]", S);
+    NR_UNSUPPORTED(S < 1, "mhsa: sequence length %d", S);
     const int dhp = pick_dhp(dh);
     NR_UNSUPPORTED(dhp == 0, "mhsa: head dim %d > 128", dh);
     const size_t lds = (size_t)(2 * S * dhp + S * (dhp + 1) + S * (S + 1) + S) * sizeof(float);
-    NR_UNSUPPORTED(lds > MHSA_LDS_MAX, "mhsa: S=%d with head dim %d needs %zu B of LDS (> %zu)", S, dh, lds, MHSA_LDS_MAX);
+    if (S > 128 || lds > MHSA_LDS_MAX) return mhsa_long_fwd(qkv, mask, ctx, row_max, row_sum, N, S, H, dh, dc, s);
     ProfScope prof(FAM_ATTN, s, 4.0 * N * H * S * S * dh);
     const dim3 grid((unsigned)(N * H));
 #define NR_FWD(P, T)                                                                                                \
@@ -381,9 +418,10 @@ int mhsa_bwd(const float* qkv, const int64_t* mask, const float* ctx, const floa
         return mhsa_bwd_mfma2(qkv, mask, dctx, row_max, row_sum, dqkv, N, S, H, dh, dc, s);
     }
     NR_UNSUPPORTED(dc.offs != nullptr, "mhsa bwd: packed sequences need S <= 32 and head dim <= 64 (got S=%d, dh=%d; 32 < S <= 64 is packed in the forward only)", S, dh);
-    NR_UNSUPPORTED(S > 128 || S < 1, "mhsa bwd: sequence length %d not in [1,128]", S);
+    NR_UNSUPPORTED(S < 1, "mhsa bwd: sequence length %d", S);
     const int dhp = pick_dhp(dh);
-    NR_UNSUPPORTED(dhp == 0 || dhp > 64, "mhsa bwd: head dim %d > 64", dh);
+    NR_UNSUPPORTED(dhp == 0, "mhsa bwd: head dim %d > 128", dh);
+    if (S > 128 || dhp > 64) return mhsa_long_bwd(qkv, mask, ctx, dctx, row_max, row_sum, dqkv, N, S, H, dh, dc, s);
     size_t lds = (size_t)(2 * S * dhp + 3 * S * (dhp + 1) + 2 * S * (S + 1) + S) * sizeof(float);
     ProfScope prof(FAM_ATTN, s, 10.0 * N * H * S * S * dh);
     const dim3 grid((unsigned)(N * H));

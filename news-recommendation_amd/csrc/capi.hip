@@ -3,6 +3,7 @@
 #include "gemm.h"
 #include "rowops.h"
 #include "seqops.h"
+#include "attention_long.h"
 #include "../../include/newsrec_hip.h"
 
 #include <stdarg.h>
@@ -464,6 +465,65 @@ int nr_mhsa_bwd_bf16(const void* qkv, const int64_t* mask, const void* dctx, con
     NR_CHECK_ARG(N >= 0 && Sq > 0 && H > 0 && dh > 0, "mhsa_bwd_bf16: bad sizes");
     NR_CHECK_ARG(N == 0 || (qkv && mask && dctx && row_max && row_sum && dqkv), "mhsa_bwd_bf16: null pointer");
     return mhsa_bwd_mfma_h((const unsigned short*)qkv, mask, (const unsigned short*)dctx, row_max, row_sum, (unsigned short*)dqkv, N, (int)Sq, (int)H, (int)dh, DCA(p_drop, seed, site, mask_mode), S(stream));
+}
+
+// ---- softmax attention of any length
+static int attn_problem(const nr_attention* p, AttnProblem* a, const char* what) {
+    NR_CHECK_ARG(p, "%s: null problem", what);
+    NR_CHECK_ARG(p->N >= 0 && p->Sq >= 0 && p->Sk >= 0 && p->H > 0 && p->G > 0 && p->dh > 0, "%s: bad sizes", what);
+    NR_CHECK_ARG(p->H % p->G == 0, "%s: %lld query heads are not a multiple of %lld key heads", what, (long long)p->H, (long long)p->G);
+    NR_CHECK_ARG(p->dtype == 0 || p->dtype == 1, "%s: dtype %d is neither 0 (fp32) nor 1 (bf16)", what, p->dtype);
+    NR_CHECK_ARG(p->p_drop >= 0.f && p->p_drop < 1.f, "%s: p_drop %f not in [0,1)", what, p->p_drop);
+    NR_CHECK_ARG(p->scale > 0.f && p->scale < INFINITY, "%s: scale %f is not a positive number", what, p->scale);
+    NR_UNSUPPORTED(p->dh > 128, "%s: head dim %lld > 128", what, (long long)p->dh);
+    NR_UNSUPPORTED(p->Sk > 0x3fffffff || p->H / p->G * p->Sq > 0x3fffffff, "%s: %lld keys or %lld rows per key head exceed 2^30", what, (long long)p->Sk, (long long)(p->H / p->G * p->Sq));
+    if (p->N == 0 || p->Sq == 0) return NR_OK;
+    NR_CHECK_ARG(p->q && (p->Sk == 0 || (p->k && p->v)), "%s: null pointer", what);
+    a->q = p->q; a->k = p->k; a->v = p->v; a->key_mask = p->key_mask;
+    a->sq = {p->q_stride[0], p->q_stride[1], p->q_stride[2]};
+    a->sk = {p->k_stride[0], p->k_stride[1], p->k_stride[2]};
+    a->sv = {p->v_stride[0], p->v_stride[1], p->v_stride[2]};
+    a->N = p->N; a->Sq = (int)p->Sq; a->Sk = (int)p->Sk; a->H = (int)p->H; a->G = (int)p->G; a->dh = (int)p->dh;
+    a->bf16 = p->dtype == 1; a->causal = p->causal != 0; a->scale = p->scale;
+    a->dc = DCA(p->p_drop, p->seed, p->site, 1);
+    return NR_OK;
+}
+static AttnStrides dense(int64_t S, int64_t H, int64_t dh) { return {S * H * dh, H * dh, dh}; }
+
+size_t nr_attention_fwd_ws_bytes(const nr_attention* p) {
+    AttnProblem a;
+    return attn_problem(p, &a, "attention_fwd") == NR_OK && a.N ? attn_long_fwd_ws_bytes(a) : 0;
+}
+int nr_attention_fwd(const nr_attention* p, void* out, float* row_max, float* row_sum, void* ws, size_t ws_bytes, void* stream) {
+    AttnProblem a;
+    if (int rc = attn_problem(p, &a, "attention_fwd")) return rc;
+    if (a.N == 0) return NR_OK;
+    NR_CHECK_ARG(out, "attention_fwd: null pointer");
+    NR_CHECK_ARG((row_max == nullptr) == (row_sum == nullptr), "attention_fwd: row_max/row_sum must both be given or both NULL");
+    if (ws_bytes < attn_long_fwd_ws_bytes(a) || (!ws && attn_long_fwd_ws_bytes(a))) { set_error("attention_fwd: workspace too small"); return NR_ERR_WORKSPACE; }
+    AttnOut o;
+    o.out = out; o.so = dense(a.Sq, a.H, a.dh); o.row_max = row_max; o.row_sum = row_sum;
+    ProfScope prof(FAM_ATTN, S(stream), 4.0 * a.N * a.H * a.Sq * a.Sk * a.dh);
+    return attn_long_fwd(a, o, ws, ws_bytes, S(stream));
+}
+size_t nr_attention_bwd_ws_bytes(const nr_attention* p) {
+    AttnProblem a;
+    return attn_problem(p, &a, "attention_bwd") == NR_OK && a.N && a.Sk ? attn_long_bwd_ws_bytes(a) : 0;
+}
+int nr_attention_bwd(const nr_attention* p, const void* out, const void* dout, const float* row_max, const float* row_sum, float* delta, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream) {
+    AttnProblem a;
+    if (int rc = attn_problem(p, &a, "attention_bwd")) return rc;
+    NR_CHECK_ARG(a.N == 0 || a.Sk > 0, "attention_bwd: no keys (every gradient is zero: nothing to compute)");
+    if (a.N == 0) return NR_OK;
+    NR_CHECK_ARG(out && dout && row_max && row_sum && delta && dq && dk && dv, "attention_bwd: null pointer");
+    if (ws_bytes < attn_long_bwd_ws_bytes(a) || (!ws && attn_long_bwd_ws_bytes(a))) { set_error("attention_bwd: workspace too small"); return NR_ERR_WORKSPACE; }
+    AttnGrad g;
+    g.out = out; g.dout = dout; g.so = g.sdo = g.sdq = dense(a.Sq, a.H, a.dh);
+    g.row_max = row_max; g.row_sum = row_sum;
+    g.delta = delta; g.sd = {(int64_t)a.H * a.Sq, 1, a.Sq};
+    g.dq = dq; g.dk = dk; g.dv = dv; g.sdk = g.sdv = dense(a.Sk, a.G, a.dh);
+    ProfScope prof(FAM_ATTN, S(stream), 10.0 * a.N * a.H * a.Sq * a.Sk * a.dh);
+    return attn_long_bwd(a, g, ws, ws_bytes, S(stream));
 }
 
 int nr_query_pool_fwd_f32(const float* key, const float* value, const float* table, const int64_t* idx, int64_t table_rows, const float* query, const int64_t* mask, int64_t nseq, int64_t Sq, int64_t D, float* out, float* prob, void* stream) {

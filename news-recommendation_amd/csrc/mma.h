@@ -1,0 +1,132 @@
+// 32x32 matrix-core tiles over one element type, for kernels that run the same tiling on fp32 and on bf16 tensors
+// (attention_long.hip, linear_attention.hip).
+//
+// A product D[i][j] += sum_k A[i][k] B[k][j] is taken in k-steps of 16.  A lane (l = lane & 31, h = lane >> 5) holds 8 of the 16
+// k's of row i = l of A and of column j = l of B ("fragment"), and 16 elements of D: column j = l, rows
+// row(r, h) = (r & 3) + 8 * (r >> 2) + 4 * h.  WHICH 8 of the k's a lane half holds is free as long as A and B agree; two orders
+// are used:
+//   "near":  k = 8 h + e                        (operands read as 8 consecutive elements of a row)
+//   "tile":  k = 4 h + (e & 3) + 8 * (e >> 2)   (operands that are D tiles of an earlier product: element e of k-step kb is
+//                                                register 8 kb + e, so a D tile feeds the next product without leaving the lane)
+// bf16: one v_mfma_f32_32x32x16_bf16 per k-step.  fp32: eight v_mfma_f32_32x32x2_f32, the e-th on element e of both fragments
+// (its two k's are the halves' e-th elements); full fp32 products and sums at the fp32 matrix rate.
+#pragma once
+#include "common.h"
+
+namespace nr {
+namespace mma {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <class T> struct Ty;
+template <> struct Ty<float> {
+    typedef f32x8 Frag;
+    static constexpr int E = 4;        // elements per 16 bytes
+    static constexpr int PAD = 4;      // LDS pitch = padded width + PAD: 16-byte rows whose starts walk over the banks
+};
+template <> struct Ty<__bf16> {
+    typedef bf16x8 Frag;
+    static constexpr int E = 8;
+    static constexpr int PAD = 8;
+};
+
+__device__ __forceinline__ int tile_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+__device__ __forceinline__ f32x16 mul(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mul(const f32x8& a, const f32x8& b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+// 8 consecutive elements of an LDS row ("near" order: p already points at column 16 * kstep + 8 * h)
+__device__ __forceinline__ bf16x8 near_frag(const __bf16* p) { return *reinterpret_cast<const bf16x8*>(p); }
+__device__ __forceinline__ f32x8 near_frag(const float* p) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// column col0 + l of the LDS tile, rows row0 + ("tile" order).  bf16: two transposed 8-byte reads, each handing lane i of a
+// 16-lane group column i of a 4-row block whose rows the group's lanes 4 q + p address (row q, columns 4 p ..): EXEC must be
+// all ones.
+template <int PITCH>
+__device__ __forceinline__ bf16x8 col_frag(const __bf16* tile, int row0, int col0, int lane) {
+    const int g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3;
+    const __bf16* z = tile + (row0 + 4 * (g >> 1) + q) * PITCH + col0 + 16 * (g & 1) + 4 * p;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(z));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(z + 8 * PITCH));
+    return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+}
+template <int PITCH>
+__device__ __forceinline__ f32x8 col_frag(const float* tile, int row0, int col0, int lane) {
+    const float* z = tile + (row0 + 4 * (lane >> 5)) * PITCH + col0 + (lane & 31);
+    return f32x8{z[0], z[PITCH], z[2 * PITCH], z[3 * PITCH], z[8 * PITCH], z[9 * PITCH], z[10 * PITCH], z[11 * PITCH]};
+}
+
+// registers 8 kb .. 8 kb + 7 of a D tile as a fragment in "tile" order (bf16: rounded to nearest even)
+template <class T> __device__ __forceinline__ typename Ty<T>::Frag tile_frag(const f32x16& t, int kb) {
+    typename Ty<T>::Frag o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (T)t[8 * kb + e];
+    return o;
+}
+
+// E consecutive elements of a global row as one 16-byte word; elements at and past `n` are zero.  VEC: the address is a multiple
+// of 16 and n is a multiple of E.
+template <class T, bool VEC>
+__device__ __forceinline__ u32x4 load16(const T* p, int n) {
+    if (n <= 0) return u32x4{0, 0, 0, 0};
+    if (VEC) return *reinterpret_cast<const u32x4*>(p);
+    if (sizeof(T) == 4) {
+        u32x4 o = {0, 0, 0, 0};
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (e < n) o[e] = w[e];
+        return o;
+    }
+    uint32_t s[8];
+    const uint16_t* w = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = e < n ? w[e] : 0;
+    return u32x4{s[0] | s[1] << 16, s[2] | s[3] << 16, s[4] | s[5] << 16, s[6] | s[7] << 16};
+}
+// a whole fragment (8 consecutive elements, "near" order) from global memory
+template <bool VEC> __device__ __forceinline__ bf16x8 load_frag(const __bf16* p, int n) {
+    return __builtin_bit_cast(bf16x8, load16<__bf16, VEC>(p, n));
+}
+template <bool VEC> __device__ __forceinline__ f32x8 load_frag(const float* p, int n) {
+    const f32x4 a = __builtin_bit_cast(f32x4, load16<float, VEC>(p, n));
+    const f32x4 b = __builtin_bit_cast(f32x4, load16<float, VEC>(p + 4, n - 4));
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+// four consecutive elements (registers 4 i .. 4 i + 3 of a D tile whose rows run along the output's last axis)
+template <bool VEC> __device__ __forceinline__ void store4(__bf16* p, const f32x4& v, int n) {
+    bf16x4 o = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    if (VEC) { if (n > 0) *reinterpret_cast<bf16x4*>(p) = o; return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (e < n) p[e] = o[e];
+}
+template <bool VEC> __device__ __forceinline__ void store4(float* p, const f32x4& v, int n) {
+    if (VEC) { if (n > 0) *reinterpret_cast<f32x4*>(p) = v; return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (e < n) p[e] = v[e];
+}
+
+}  // namespace mma
+}  // namespace nr

@@ -42,6 +42,12 @@ class TfmSavedBf16(C.Structure):
     _fields_ = [(n, c_fp) for n in ("x_h", "qkv_h", "ctx_h", "y1_h", "z_h", "a_h", "s1", "y1", "s2", "stats", "row_max", "row_sum", "w_h", "wT_h")]
 
 
+class Attention(C.Structure):
+    _fields_ = ([(n, c_fp) for n in ("q", "k", "v", "key_mask")] + [(n, c_i64) for n in ("N", "Sq", "Sk", "H", "G", "dh")] +
+                [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")] +
+                [("dtype", C.c_int32), ("causal", C.c_int32), ("scale", c_f), ("p_drop", c_f), ("seed", c_u64), ("site", c_u32)])
+
+
 _SIGS = {
     "nr_version": (c_int, []),
     "nr_last_error": (C.c_char_p, []),
@@ -77,6 +83,10 @@ _SIGS = {
     "nr_mhsa_bwd_bf16": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_i64, c_f, c_u64, c_u32, c_int, c_fp, c_fp]),
     "nr_mhsa_bwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_i64, c_f, c_u64, c_u32, c_int,
                                 c_fp, c_fp]),
+    "nr_attention_fwd_ws_bytes": (c_sz, [C.POINTER(Attention)]),
+    "nr_attention_fwd": (c_int, [C.POINTER(Attention), c_fp, c_fp, c_fp, c_fp, c_sz, c_fp]),
+    "nr_attention_bwd_ws_bytes": (c_sz, [C.POINTER(Attention)]),
+    "nr_attention_bwd": (c_int, [C.POINTER(Attention)] + [c_fp] * 9 + [c_sz, c_fp]),
     "nr_query_pool_fwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_i64, c_fp, c_fp, c_i64, c_i64, c_i64, c_fp, c_fp, c_fp]),
     "nr_query_pool_bwd_ws_bytes": (c_sz, [c_i64, c_i64]),
     "nr_query_pool_bwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_int, c_int,

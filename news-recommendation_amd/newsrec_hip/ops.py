@@ -5,15 +5,17 @@ stream and autograd's graph.  Every number is produced by the HIP kernels; a
 tensor that is not a contiguous fp32/int64 tensor on a ROCm device is an
 error, not a cue to fall back (there is nothing to fall back to).
 """
+import contextlib
 import ctypes as C
 import math
 import os
 import time
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
+from ._lib import Attention, NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
 
 PAD_ID = 0          # BERT word_embeddings.padding_idx (manager.special_token_ids["[PAD]"])
 LN_EPS = 1e-12      # models/modules/attention.py:106,151 of the reference
@@ -460,6 +462,117 @@ def mhsa(qkv, mask, N, S, H, dh, p_drop=0.0, seed=0, site=0, hf_mask=False):
     """qkv [N*S, 3*H*dh] (q | k | v per row), mask [N,S] 0/1 -> context [N*S, H*dh]"""
     return _MHSA.apply(_f32(qkv, "qkv"), _i64(mask, "attention_mask"), int(N), int(S), int(H), int(dh), float(p_drop), int(seed),
                        int(site), 1 if hf_mask else 0)
+
+
+# ----------------------------------------------------------------------------- attention of any length
+_SEQ_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _seq(t, name, dims, like=None):
+    """fp32 / bf16 tensor of `dims` axes with a dense innermost one, on a ROCm device (that of `like`, and of its type)"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise NewsrecError(f"{name}: the MI355X HIP path needs a tensor on a ROCm device "
+                           f"(got {type(t).__name__} on {getattr(t, 'device', None)}); there is no CPU path in this package")
+    if t.dtype not in _SEQ_TYPES:
+        raise NewsrecError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() != dims:
+        raise NewsrecError(f"{name}: expected {dims} axes, got {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise NewsrecError(f"{name}: {t.dtype} on {t.device}, but the other operands are {like.dtype} on {like.device}")
+    return t if t.numel() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _same_device(t, name, device):
+    if t is not None and t.device != device:
+        raise NewsrecError(f"{name}: on {t.device}, but the other operands are on {device}")
+    return t
+
+
+def _on_device(t):
+    """the kernels run on the current device's current stream: make `t`'s device the current one"""
+    if _cur_device is not None and _cur_device() == t.device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _attention_problem(q, k, v, mask, causal, scale, p, seed, site):
+    (N, Sq, H, dh), (Sk, G) = q.shape, k.shape[1:3]
+    three = C.c_int64 * 3
+    return Attention(_p(q), _p(k), _p(v), _p(mask), N, Sq, Sk, H, G, dh, three(*q.stride()[:3]), three(*k.stride()[:3]), three(*v.stride()[:3]),
+                     _SEQ_TYPES[q.dtype], int(causal), scale, p, seed, site)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, causal, scale, p, seed, site, grad_mode):
+        N, Sq, H, dh = q.shape
+        out = torch.empty(N, Sq, H, dh, dtype=q.dtype, device=q.device)
+        ctx.set_materialize_grads(False)
+        ctx.cfg = (causal, scale, p, seed, site)
+        if out.numel() == 0 or k.shape[1] == 0:
+            ctx.save_for_backward(q, k, v, mask, None, None, None)
+            return out.zero_()
+        train = grad_mode and any(ctx.needs_input_grad[:3])      # (see _TFMLayer.forward)
+        rmax = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device) if train else None
+        rsum = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device) if train else None
+        L = lib()
+        with _on_device(q):
+            P = _attention_problem(q, k, v, mask, *ctx.cfg)
+            nbytes = L.nr_attention_fwd_ws_bytes(C.byref(P))
+            ws = _ws(nbytes, q.device) if nbytes else None
+            check(L.nr_attention_fwd(C.byref(P), _p(out), _p(rmax), _p(rsum), _p(ws), nbytes, _stream()), "nr_attention_fwd")
+        if train:
+            ctx.save_for_backward(q, k, v, mask, out, rmax, rsum)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        if g is None:
+            return (None,) * 10
+        q, k, v, mask, out, rmax, rsum = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if out is None:
+            return (dq.zero_(), dk.zero_(), dv.zero_()) + (None,) * 7
+        g = g.contiguous()
+        N, Sq, H, _ = q.shape
+        delta = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device)
+        L = lib()
+        with _on_device(q):
+            P = _attention_problem(q, k, v, mask, *ctx.cfg)
+            nbytes = L.nr_attention_bwd_ws_bytes(C.byref(P))
+            ws = _ws(nbytes, q.device) if nbytes else None
+            check(L.nr_attention_bwd(C.byref(P), _p(out), _p(g), _p(rmax), _p(rsum), _p(delta), _p(dq), _p(dk), _p(dv), _p(ws), nbytes,
+                                     _stream()), "nr_attention_bwd")
+        return (dq, dk, dv) + (None,) * 7
+
+
+def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed=0, site=0):
+    """softmax(scale * q k^T) v per head for sequences of any length (nr_attention_fwd / _bwd): q [N,Sq,H,dh], k / v [N,Sk,G,dh]
+    -> [N,Sq,H,dh]; fp32 or bf16, dh <= 128, any strides with a dense innermost axis (the blocks of one [N,S,3,H,dh] projection
+    are read where they are).  H a multiple of G: query head h reads key head h // (H // G).  key_mask [N,Sk] 0/1 or bool: keys
+    with 0 do not take part, whatever their rows hold.  causal: query i sees the keys up to i + Sk - Sq.  A query without a key
+    gives a zero row and sends no gradient.  scale: a positive number, default 1 / sqrt(dh).  p_drop: dropout on the
+    probabilities from the library's stream (seed, site)."""
+    q = _seq(q, "q", 4)
+    k, v = _seq(k, "k", 4, q), _seq(v, "v", 4, q)
+    N, Sq, H, dh = q.shape
+    if k.shape != v.shape or k.shape[0] != N or k.shape[3] != dh:
+        raise NewsrecError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if H == 0 or dh == 0 or k.shape[2] == 0 or H % k.shape[2]:
+        raise NewsrecError(f"attention: {H} query heads of width {dh} over {k.shape[2]} key heads")
+    if dh > 128:
+        raise NewsrecError(f"attention: head dim {dh} > 128")
+    if key_mask is not None:
+        key_mask = _same_device(_i64(key_mask, "key_mask"), "key_mask", q.device)
+        if tuple(key_mask.shape) != (N, k.shape[1]):
+            raise NewsrecError(f"attention: key_mask {tuple(key_mask.shape)} for {N} sequences of {k.shape[1]} keys")
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise NewsrecError(f"attention: scale {scale} is not a positive number")
+    if not 0.0 <= p_drop < 1.0:
+        raise NewsrecError(f"attention: p_drop {p_drop} not in [0, 1)")
+    return _Attention.apply(q, k, v, key_mask, bool(causal), scale, float(p_drop), int(seed), int(site), torch.is_grad_enabled())
 
 
 # ----------------------------------------------------------------------------- conv1d(k=3, pad=1) + relu
