@@ -181,6 +181,32 @@ int nr_attention_fwd(const nr_attention* p, void* out, float* row_max, float* ro
 size_t nr_attention_bwd_ws_bytes(const nr_attention* p);
 int nr_attention_bwd(const nr_attention* p, const void* out, const void* dout, const float* row_max, const float* row_sum, float* delta, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- linear attention with a decay for each head --------------------------------------------------------------------
+ * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  out_t = scale * q_t S_t  for the tokens t < lens[n] of every sequence (lens [N] int64,
+ * taken into [0, S]; NULL: all S): a recurrent user tower beside nr_gru_fwd_f32 (RnnUserEncoder, encoder.py:204-233) whose tokens
+ * do not wait for each other.  out rows behind a sequence's length are zero; what q / k / v hold there is never used.
+ * q / k [N,S,H,dk], v [N,S,H,dv]: dtype 0 = fp32, 1 = bf16, innermost axis dense, other strides in elements; dk, dv <= 128.
+ * log_decay [H] fp32, <= 0 (-INFINITY: no memory) and, like lens, not differentiated.  state / last [N,H,dk,dv] fp32, dense: the
+ * state before the first and after the last token (state NULL: zero; last must be given).  out [N,S,H,dv] dense.
+ * bwd: dout like out; dlast the gradient of last (NULL: zero); dq / dk / dv dense; dstate the gradient of state (NULL: not wanted).
+ * Fixed summation order: the same bits every time.  ws: nr_linear_attention_{fwd,bwd}_ws_bytes(p) bytes, scratch of this call. */
+typedef struct {
+    const void *q, *k, *v;
+    const float *log_decay;
+    const int64_t *lens;
+    const float *state;
+    int64_t N, S, H, dk, dv;
+    int64_t q_stride[3], k_stride[3], v_stride[3];      /* sequence, position, head */
+    int32_t dtype;
+    float scale;
+} nr_linear_attention;
+size_t nr_linear_attention_fwd_ws_bytes(const nr_linear_attention* p);
+int nr_linear_attention_fwd(const nr_linear_attention* p, void* out, float* last, void* ws, size_t ws_bytes, void* stream);
+size_t nr_linear_attention_bwd_ws_bytes(const nr_linear_attention* p);
+int nr_linear_attention_bwd(const nr_linear_attention* p, const void* dout, const float* dlast, void* dq, void* dk, void* dv, float* dstate, void* ws, size_t ws_bytes, void* stream);
+/* one token of the same recurrence: q / k [N,H,dk], v [N,H,dv], out [N,H,dv] dense; out_state may be state (updated in place) */
+int nr_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state, int64_t N, int64_t H, int64_t dk, int64_t dv, int dtype, float scale, void* out, float* out_state, void* stream);
+
 /* ---- additive ("query") pooling — scaled_dp_attention, attention.py:6-34 -----------------------
  * out[n,:] = softmax_s(query . key[n,s,:] / sqrt(D) + (1-mask[n,s]) * -1e5) . value[n,s,:]
  * key/value [nseq,S,D]; if idx != NULL, key and value rows are table[idx[n,s],:] instead (eval:

@@ -4,8 +4,10 @@
 #include "rowops.h"
 #include "seqops.h"
 #include "attention_long.h"
+#include "linear_attention.h"
 #include "../../include/newsrec_hip.h"
 
+#include <math.h>
 #include <stdarg.h>
 #include <cstdlib>
 #include <atomic>
@@ -524,6 +526,60 @@ int nr_attention_bwd(const nr_attention* p, const void* out, const void* dout, c
     g.dq = dq; g.dk = dk; g.dv = dv; g.sdk = g.sdv = dense(a.Sk, a.G, a.dh);
     ProfScope prof(FAM_ATTN, S(stream), 10.0 * a.N * a.H * a.Sq * a.Sk * a.dh);
     return attn_long_bwd(a, g, ws, ws_bytes, S(stream));
+}
+
+// ---- linear attention with a decay for each head
+static int lin_sizes(const char* what, int64_t N, int64_t S, int64_t H, int64_t dk, int64_t dv, int dtype, float scale) {
+    NR_CHECK_ARG(N >= 0 && S >= 0 && H > 0 && dk > 0 && dv > 0, "%s: bad sizes", what);
+    NR_CHECK_ARG(dtype == 0 || dtype == 1, "%s: dtype %d is neither 0 (fp32) nor 1 (bf16)", what, dtype);
+    NR_CHECK_ARG(fabsf(scale) < INFINITY, "%s: scale %f is not a number", what, scale);
+    NR_UNSUPPORTED(dk > 128 || dv > 128, "%s: head dims %lld, %lld > 128", what, (long long)dk, (long long)dv);
+    NR_UNSUPPORTED(S > 0x3fffffff || H > 0xffff, "%s: %lld tokens or %lld heads", what, (long long)S, (long long)H);
+    return NR_OK;
+}
+static int lin_problem(const nr_linear_attention* p, LinProblem* a, const char* what) {
+    NR_CHECK_ARG(p, "%s: null problem", what);
+    if (int rc = lin_sizes(what, p->N, p->S, p->H, p->dk, p->dv, p->dtype, p->scale)) return rc;
+    if (p->N == 0) return NR_OK;
+    NR_CHECK_ARG(p->log_decay && (p->S == 0 || (p->q && p->k && p->v)), "%s: null pointer", what);
+    a->q = p->q; a->k = p->k; a->v = p->v; a->log_decay = p->log_decay; a->lens = p->lens; a->state = p->state;
+    a->sq = {p->q_stride[0], p->q_stride[1], p->q_stride[2]};
+    a->sk = {p->k_stride[0], p->k_stride[1], p->k_stride[2]};
+    a->sv = {p->v_stride[0], p->v_stride[1], p->v_stride[2]};
+    a->N = p->N; a->S = (int)p->S; a->H = (int)p->H; a->dk = (int)p->dk; a->dv = (int)p->dv;
+    a->bf16 = p->dtype == 1; a->scale = p->scale;
+    return NR_OK;
+}
+size_t nr_linear_attention_fwd_ws_bytes(const nr_linear_attention* p) {
+    LinProblem a;
+    return lin_problem(p, &a, "linear_attention_fwd") == NR_OK && a.N ? lin_fwd_ws_bytes(a) : 0;
+}
+int nr_linear_attention_fwd(const nr_linear_attention* p, void* out, float* last, void* ws, size_t ws_bytes, void* stream) {
+    LinProblem a;
+    if (int rc = lin_problem(p, &a, "linear_attention_fwd")) return rc;
+    if (a.N == 0) return NR_OK;
+    NR_CHECK_ARG((out || a.S == 0) && last, "linear_attention_fwd: null pointer");
+    ProfScope prof(FAM_ATTN, S(stream), 4.0 * a.N * a.H * a.S * a.dk * a.dv);
+    return lin_fwd(a, out, last, ws, ws_bytes, S(stream));
+}
+size_t nr_linear_attention_bwd_ws_bytes(const nr_linear_attention* p) {
+    LinProblem a;
+    return lin_problem(p, &a, "linear_attention_bwd") == NR_OK && a.N ? lin_bwd_ws_bytes(a) : 0;
+}
+int nr_linear_attention_bwd(const nr_linear_attention* p, const void* dout, const float* dlast, void* dq, void* dk, void* dv, float* dstate, void* ws, size_t ws_bytes, void* stream) {
+    LinProblem a;
+    if (int rc = lin_problem(p, &a, "linear_attention_bwd")) return rc;
+    if (a.N == 0) return NR_OK;
+    NR_CHECK_ARG(a.S == 0 || (dout && dq && dk && dv), "linear_attention_bwd: null pointer");
+    ProfScope prof(FAM_ATTN, S(stream), 10.0 * a.N * a.H * a.S * a.dk * a.dv);
+    return lin_bwd(a, dout, dlast, dq, dk, dv, dstate, ws, ws_bytes, S(stream));
+}
+int nr_linear_attention_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state, int64_t N, int64_t H, int64_t dk, int64_t dv, int dtype, float scale, void* out, float* out_state, void* stream) {
+    if (int rc = lin_sizes("linear_attention_step", N, 1, H, dk, dv, dtype, scale)) return rc;
+    if (N == 0) return NR_OK;
+    NR_CHECK_ARG(q && k && v && log_decay && state && out && out_state, "linear_attention_step: null pointer");
+    ProfScope prof(FAM_ATTN, S(stream), 5.0 * N * H * dk * dv);
+    return lin_step(q, k, v, log_decay, state, N, (int)H, (int)dk, (int)dv, dtype == 1, scale, out, out_state, S(stream));
 }
 
 int nr_query_pool_fwd_f32(const float* key, const float* value, const float* table, const int64_t* idx, int64_t table_rows, const float* query, const int64_t* mask, int64_t nseq, int64_t Sq, int64_t D, float* out, float* prob, void* stream) {

@@ -48,6 +48,11 @@ class Attention(C.Structure):
                 [("dtype", C.c_int32), ("causal", C.c_int32), ("scale", c_f), ("p_drop", c_f), ("seed", c_u64), ("site", c_u32)])
 
 
+class LinearAttention(C.Structure):
+    _fields_ = ([(n, c_fp) for n in ("q", "k", "v", "log_decay", "lens", "state")] + [(n, c_i64) for n in ("N", "S", "H", "dk", "dv")] +
+                [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("dtype", C.c_int32), ("scale", c_f)])
+
+
 _SIGS = {
     "nr_version": (c_int, []),
     "nr_last_error": (C.c_char_p, []),
@@ -87,6 +92,11 @@ _SIGS = {
     "nr_attention_fwd": (c_int, [C.POINTER(Attention), c_fp, c_fp, c_fp, c_fp, c_sz, c_fp]),
     "nr_attention_bwd_ws_bytes": (c_sz, [C.POINTER(Attention)]),
     "nr_attention_bwd": (c_int, [C.POINTER(Attention)] + [c_fp] * 9 + [c_sz, c_fp]),
+    "nr_linear_attention_fwd_ws_bytes": (c_sz, [C.POINTER(LinearAttention)]),
+    "nr_linear_attention_fwd": (c_int, [C.POINTER(LinearAttention), c_fp, c_fp, c_fp, c_sz, c_fp]),
+    "nr_linear_attention_bwd_ws_bytes": (c_sz, [C.POINTER(LinearAttention)]),
+    "nr_linear_attention_bwd": (c_int, [C.POINTER(LinearAttention)] + [c_fp] * 7 + [c_sz, c_fp]),
+    "nr_linear_attention_step": (c_int, [c_fp] * 5 + [c_i64] * 4 + [c_int, c_f, c_fp, c_fp, c_fp]),
     "nr_query_pool_fwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_i64, c_fp, c_fp, c_i64, c_i64, c_i64, c_fp, c_fp, c_fp]),
     "nr_query_pool_bwd_ws_bytes": (c_sz, [c_i64, c_i64]),
     "nr_query_pool_bwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_int, c_int,

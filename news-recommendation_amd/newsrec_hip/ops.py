@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import Attention, NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
+from ._lib import Attention, LinearAttention, NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
 
 PAD_ID = 0          # BERT word_embeddings.padding_idx (manager.special_token_ids["[PAD]"])
 LN_EPS = 1e-12      # models/modules/attention.py:106,151 of the reference
@@ -848,6 +848,114 @@ def gru_final_state(x, mask, w_ih, w_hh, b_ih, b_hh):
         raise NewsrecError(f"gru_final_state: x {tuple(x.shape)} / mask {tuple(mask.shape)} shape mismatch")
     return _GRUFinal.apply(x, mask, _f32(w_ih, "rnn.weight_ih_l0"), _f32(w_hh, "rnn.weight_hh_l0"), _f32(b_ih, "rnn.bias_ih_l0"),
                            _f32(b_hh, "rnn.bias_hh_l0"), torch.is_grad_enabled())
+
+
+# ----------------------------------------------------------------------------- linear attention with a decay per head
+def _linear_problem(q, k, v, log_decay, lens, state, scale):
+    (N, S, H, dk), dv = q.shape, v.shape[3]
+    three = C.c_int64 * 3
+    return LinearAttention(_p(q), _p(k), _p(v), _p(log_decay), _p(lens), _p(state), N, S, H, dk, dv, three(*q.stride()[:3]),
+                           three(*k.stride()[:3]), three(*v.stride()[:3]), _SEQ_TYPES[q.dtype], scale)
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, lens, state, scale):
+        (N, S, H, dk), dv = q.shape, v.shape[3]
+        out = torch.empty(N, S, H, dv, dtype=q.dtype, device=q.device)
+        last = torch.empty(N, H, dk, dv, dtype=torch.float32, device=q.device)
+        L = lib()
+        with _on_device(q):
+            P = _linear_problem(q, k, v, log_decay, lens, state, scale)
+            nbytes = L.nr_linear_attention_fwd_ws_bytes(C.byref(P))
+            ws = _ws(nbytes, q.device) if nbytes else None
+            check(L.nr_linear_attention_fwd(C.byref(P), _p(out), _p(last), _p(ws), nbytes, _stream()), "nr_linear_attention_fwd")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, lens, state)
+        ctx.scale = scale
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, glast):
+        q, k, v, log_decay, lens, state = ctx.saved_tensors
+        if g is None and glast is None:
+            return (None,) * 7
+        (N, S, H, dk), dv = q.shape, v.shape[3]
+        g = torch.zeros(N, S, H, dv, dtype=q.dtype, device=q.device) if g is None else g.contiguous()
+        glast = None if glast is None else glast.contiguous()
+        dq, dk_, dv_ = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dstate = torch.empty(N, H, dk, dv, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[5] else None
+        L = lib()
+        with _on_device(q):
+            P = _linear_problem(q, k, v, log_decay, lens, state, ctx.scale)
+            nbytes = L.nr_linear_attention_bwd_ws_bytes(C.byref(P))
+            ws = _ws(nbytes, q.device) if nbytes else None
+            check(L.nr_linear_attention_bwd(C.byref(P), _p(g), _p(glast), _p(dq), _p(dk_), _p(dv_), _p(dstate), _p(ws), nbytes, _stream()),
+                  "nr_linear_attention_bwd")
+        return dq, dk_, dv_, None, None, dstate, None
+
+
+def _linear_args(what, q, k, v, log_decay, state, scale, dims):
+    q = _seq(q, "q", dims)
+    k, v = _seq(k, "k", dims, q), _seq(v, "v", dims, q)
+    if k.shape != q.shape or v.shape[:-1] != q.shape[:-1]:
+        raise NewsrecError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    N, H, dk, dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]
+    if H == 0 or not 1 <= dk <= 128 or not 1 <= dv <= 128:
+        raise NewsrecError(f"{what}: {H} heads of widths {dk}, {dv} (1 to 128 are built)")
+    log_decay = _same_device(_f32(log_decay, "log_decay"), "log_decay", q.device)
+    if tuple(log_decay.shape) != (H,):
+        raise NewsrecError(f"{what}: log_decay {tuple(log_decay.shape)} for {H} heads")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise NewsrecError(f"{what}: log_decay is a constant of the head here, it has no gradient (detach it)")
+    if state is not None:
+        state = _same_device(_f32(state, "state"), "state", q.device)
+        if tuple(state.shape) != (N, H, dk, dv):
+            raise NewsrecError(f"{what}: state {tuple(state.shape)}, expected {(N, H, dk, dv)}")
+    scale = 1.0 / math.sqrt(dk) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise NewsrecError(f"{what}: scale {scale} is not a number")
+    return q, k, v, log_decay, state, scale
+
+
+def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
+    """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t per head (nr_linear_attention_fwd / _bwd): q / k [N,S,H,dk],
+    v [N,S,H,dv], fp32 or bf16, any strides with a dense innermost axis, widths up to 128 -> (o [N,S,H,dv], the state after the last
+    token [N,H,dk,dv] fp32).  log_decay [H] fp32, <= 0, a constant without gradient.  lens [N]: sequence n has lens[n] tokens (taken
+    into [0, S]); o is zero behind them and the state stops there.  state: the state to start from (default zero), as an earlier call
+    or linear_attention_step left it.  scale: default 1 / sqrt(dk).  Differentiable in q, k, v and state."""
+    q, k, v, log_decay, state, scale = _linear_args("linear_attention", q, k, v, log_decay, state, scale, 4)
+    if lens is not None:
+        lens = _same_device(_i64(lens, "lens"), "lens", q.device)
+        if tuple(lens.shape) != (q.shape[0],):
+            raise NewsrecError(f"linear_attention: lens {tuple(lens.shape)} for {q.shape[0]} sequences")
+    return _LinearAttention.apply(q, k, v, log_decay, lens, state, scale)
+
+
+@torch.no_grad()
+def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None):
+    """one token of linear_attention for every sequence: q / k [N,H,dk], v [N,H,dv], state [N,H,dk,dv] fp32 -> o [N,H,dv].  The new
+    state goes to out_state (dense, may be state itself), by default over state.  Inference only (no autograd)."""
+    if state is None:
+        raise NewsrecError("linear_attention_step: needs a state")
+    given = state
+    q, k, v, log_decay, state, scale = _linear_args("linear_attention_step", q, k, v, log_decay, state, scale, 3)
+    out_state = given if out_state is None else out_state
+    if (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != q.device or out_state.shape != state.shape
+            or not out_state.is_contiguous()):
+        raise NewsrecError("linear_attention_step: the state to write must be a dense fp32 tensor of the state's shape on the same device")
+    if 0 < abs(out_state.data_ptr() - state.data_ptr()) < 4 * state.numel():
+        raise NewsrecError("linear_attention_step: the state to write overlaps the state to read")
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    N, H, dk = q.shape
+    dv = v.shape[2]
+    out = torch.empty(N, H, dv, dtype=q.dtype, device=q.device)
+    with _on_device(q):
+        check(lib().nr_linear_attention_step(_p(q), _p(k), _p(v), _p(log_decay), _p(state), N, H, dk, dv, _SEQ_TYPES[q.dtype], scale, _p(out),
+                                             _p(out_state), _stream()), "nr_linear_attention_step")
+    torch.autograd.graph.increment_version(out_state)       # a graph that saved it must not take the new values for the old
+    return out
 
 
 # ----------------------------------------------------------------------------- BERT embedding stage
