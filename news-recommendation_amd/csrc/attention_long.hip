@@ -1,302 +1,10 @@
-// Softmax attention of any length: forward.
-//
-//   o_i = sum_j p_ij v_j,   p_ij = exp(x_ij - max_j x_ij) / sum_j exp(..),   x_ij = scale * q_i . k_j
-//
-// over the keys j that are there (key mask) and, causal, not behind the query (j <= i + Sk - Sq).  One pass over the keys with
-// the running maximum m and sum l of every row: a new tile's maximum m' rescales what was summed so far by exp(m - m').
-//
-// Tiling.  A workgroup of four waves takes 128 rows of one key head and walks the keys in tiles staged through LDS; a wave owns
-// 32 rows.  The query heads that share a key head are laid one below the other (row r = query head r / Sq, position r % Sq), so
-// K and V are read once for all of them.  A wave forms S^T = K Q^T (row = key, column = query): a lane then holds 16 scores of
-// ONE row per 32 keys, the softmax needs one exchange (the other lane half), and the probabilities are, register by register, the
-// B operand of O^T += V^T P^T (mma.h, "tile" order) - they never pass through LDS.
-// With at most 32 rows (a few candidates over a long history) the four waves take a quarter of every tile's keys each instead
-// (WK = 4) and meet at the end through LDS; when the workgroups do not fill the chip the keys are also split over workgroups
-// and joined by attn_join_kernel.
-//
-// Rounding: scores, maximum, sum and output are fp32; bf16 inputs round the probabilities to bf16 (the matrix instruction's
-// operand), 2^-9 each against a sum taken in fp32 from the unrounded ones.
+// Softmax attention of any length: which kernels, how split, and their launch (kernels: attention_long_fwd.h, attention_long_bwd.h)
 #include "attention_long_dev.h"
 #include <algorithm>
 
 namespace nr {
 namespace al {
 
-template <class T, int DHP, int WK> struct FwdCfg {
-    static constexpr int KSUB = (sizeof(T) == 2 && WK == 1) ? 2 : 1;     // 32-key pieces of a tile per wave
-    static constexpr int KT = 32 * KSUB * WK;
-    static constexpr int PITCH = DHP + Ty<T>::PAD;
-    static constexpr int NBUF = (sizeof(T) == 4 && DHP == 128 && WK == 4) ? 1 : 2;       // two stages where 160 KB hold them
-    static constexpr size_t LDS = (size_t)NBUF * 2 * KT * PITCH * sizeof(T);
-    static constexpr size_t JOIN = WK > 1 ? (size_t)(WK * DHP * 32 + 2 * WK * 32) * 4 : 0;
-    static constexpr size_t BYTES = LDS > JOIN ? LDS : JOIN;
-};
-
-template <class T, int DHP, bool VEC, int WK>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(const Args a) {
-    typedef FwdCfg<T, DHP, WK> C;
-    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, PITCH = C::PITCH, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
-    constexpr bool NAT = sizeof(T) == 4;         // fp32: exp(x - m) with the difference formed first (the mask's -1e5 would cost
-                                                 // a product's rounding); bf16: one fma per score in units of log 2
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + C::NBUF * KT * PITCH;
-    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wq = w / WK, wk = w % WK;
-
-    uint32_t b = xcd_order(blockIdx.x, gridDim.x);
-    const int sp = b % a.splits; b /= a.splits;
-    int rb = b % a.nblk_r; b /= a.nblk_r;
-    const int g = b % a.G;
-    const int64_t n = b / a.G;
-    if (a.causal) rb = heavy_light(rb, a.nblk_r);
-    const int r0 = rb * 32 * WQ;
-
-    // this lane's row
-    const int row = r0 + 32 * wq + l31;
-    const bool live = row < a.R;
-    const int hh = live ? row / a.Sq : 0, i = live ? row - hh * a.Sq : 0, head = g * a.rep + hh;
-    const int lim = a.causal ? i + a.Sk - a.Sq : 0x7fffffff;             // last key of the row
-    int lim_min = live ? lim : 0x7fffffff;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o, 64));
-    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    typename Ty<T>::Frag qf[KS];
-    const T* qp = static_cast<const T*>(a.q) + n * a.sq.n + i * a.sq.s + head * a.sq.h;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<VEC>(qp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
-
-    // keys of this block
-    const int begin = sp * a.per_split;
-    int end = min(a.Sk, begin + a.per_split);
-    if (a.causal) {
-        const int last = min(r0 + 32 * WQ, a.R) - 1;
-        const int imax = r0 / a.Sq == last / a.Sq ? last % a.Sq : a.Sq - 1;
-        end = min(end, imax + a.Sk - a.Sq + 1);
-    }
-    const int64_t* mask = a.mask ? a.mask + n * a.Sk : nullptr;
-    if (mask && !a.additive) end = present_end(mask, begin, end, tid);
-    const T* kp = static_cast<const T*>(a.k) + n * a.sk.n + g * a.sk.h;
-    const T* vp = static_cast<const T*>(a.v) + n * a.sv.n + g * a.sv.h;
-
-    const float scale2 = a.scale * LOG2E;
-    float m = NEVER, l = 0.f;
-    f32x16 o[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = zero16();
-
-    Stage<T, DHP, KT, VEC> sk, sv;
-    KeyBits<WORDS> kb;
-    uint64_t bits[WORDS];
-    const int tiles = end > begin ? (end - begin + KT - 1) / KT : 0;
-    auto fetch = [&](int j) {
-        kb.load(mask, j, end, lane);
-        sk.load(tid, a.dh, [&](int r) { return j + r < end ? kp + (int64_t)(j + r) * a.sk.s : nullptr; });
-        sv.load(tid, a.dh, [&](int r) { return j + r < end ? vp + (int64_t)(j + r) * a.sv.s : nullptr; });
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int x = 0; x < WORDS; ++x) bits[x] = kb.bits(x);
-        // an absent key's row reads as zero: whatever its memory holds (a NaN as well) must not reach 0 * v
-        auto keep = [&](int r) { return a.additive || ((bits[r >> 6] >> (r & 63)) & 1); };
-        sk.store(tid, Ks + buf * KT * PITCH, keep);
-        sv.store(tid, Vs + buf * KT * PITCH, keep);
-    };
-    if (tiles) { fetch(begin); put(0); }
-    __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
-        const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
-        uint64_t now[WORDS];
-#pragma unroll
-        for (int x = 0; x < WORDS; ++x) now[x] = bits[x];
-        if (t + 1 < tiles) fetch(j0 + KT);
-        const T* Kt = Ks + buf * KT * PITCH;
-        const T* Vt = Vs + buf * KT * PITCH;
-        uint32_t sub[KSUB], any = 0, all = ~0u;
-#pragma unroll
-        for (int s = 0; s < KSUB; ++s) {
-            const int ko = 32 * (wk * KSUB + s);
-            sub[s] = (uint32_t)(now[ko >> 6] >> (ko & 63));
-            any |= sub[s]; all &= sub[s];
-        }
-        const int kw = j0 + 32 * wk * KSUB;                              // first key of this wave's piece
-        if (any || (a.additive && kw < end)) {
-            f32x16 x[KSUB];
-#pragma unroll
-            for (int s = 0; s < KSUB; ++s) {
-                x[s] = zero16();
-                const T* kr = Kt + (32 * (wk * KSUB + s) + l31) * PITCH + 8 * h;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) x[s] = mul(near_frag(kr + 16 * ks), qf[ks], x[s]);
-            }
-            if (NAT) {
-#pragma unroll
-                for (int s = 0; s < KSUB; ++s) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[s][r] *= a.scale;
-                    if (a.additive) {                                    // absent keys sink by `fill`; past the end there is no key
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) if (!((sub[s] >> tile_row(r, h)) & 1)) x[s][r] += a.fill;
-                        const int left = end - kw - 32 * s;
-                        sub[s] = left >= 32 ? ~0u : (left > 0 ? (1u << left) - 1 : 0u);
-                        all = s ? all & sub[s] : sub[s];
-                    }
-                }
-            }
-            if (all != ~0u || kw + 32 * KSUB - 1 > lim_min)
-#pragma unroll
-                for (int s = 0; s < KSUB; ++s) hide(x[s], sub[s], kw + 32 * s, lim, h);
-            float top = x[0][0];
-#pragma unroll
-            for (int s = 0; s < KSUB; ++s)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, x[s][r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, NAT ? top : top * scale2);
-            if (__any(mn > m)) {
-                const float f = __builtin_amdgcn_exp2f(NAT ? (m - mn) * LOG2E : m - mn);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= f;
-                m = mn;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int s = 0; s < KSUB; ++s)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    x[s][r] = __builtin_amdgcn_exp2f(NAT ? (x[s][r] - m) * LOG2E : fmaf(x[s][r], scale2, -m));
-                    sum += x[s][r];
-                }
-            l += sum;
-            if (a.drop) {
-                const uint64_t rl = ((uint64_t)(n * a.H + head) * a.Sq + i) * a.Sk;
-#pragma unroll
-                for (int s = 0; s < KSUB; ++s)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t kp4 = keep4(a, rl + kw + 32 * s + 8 * q + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[s][4 * q + e] *= ((kp4 >> e) & 1) ? a.keep : 0.f;
-                    }
-            }
-#pragma unroll
-            for (int s = 0; s < KSUB; ++s)
-#pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                    const typename Ty<T>::Frag pf = tile_frag<T>(x[s], k2);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-                        o[d] = mul(col_frag<PITCH>(Vt, 32 * (wk * KSUB + s) + 16 * k2, 32 * d, lane), pf, o[d]);
-                }
-        }
-        if (C::NBUF == 1) __syncthreads();
-        if (t + 1 < tiles) put(C::NBUF == 2 ? 1 - buf : 0);
-        __syncthreads();
-    }
-    l += __shfl_xor(l, 32, 64);
-
-    if (WK > 1) {                                // the waves' quarters of the keys meet (in wave order: the same result every time)
-        float* slab = reinterpret_cast<float*>(smem);                    // [WK][DHP][32]
-        float* ml = slab + WK * DHP * 32;                                // [2][WK][32]
-        if (h == 0) { ml[wk * 32 + l31] = m; ml[(WK + wk) * 32 + l31] = l; }
-        __syncthreads();
-        float M = NEVER;
-#pragma unroll
-        for (int x = 0; x < WK; ++x) M = fmaxf(M, ml[x * 32 + l31]);
-        float sum = 0.f;
-#pragma unroll
-        for (int x = 0; x < WK; ++x)
-            sum += ml[(WK + x) * 32 + l31] * __builtin_amdgcn_exp2f(NAT ? (ml[x * 32 + l31] - M) * LOG2E : ml[x * 32 + l31] - M);
-        const float f = __builtin_amdgcn_exp2f(NAT ? (m - M) * LOG2E : m - M);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) slab[(wk * DHP + 32 * d + tile_row(r, h)) * 32 + l31] = o[d][r] * f;
-        __syncthreads();
-        m = M; l = sum;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q == wk % 4) {               // wave wk finishes registers 4 wk .. 4 wk + 3 of every tile
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float t = 0.f;
-#pragma unroll
-                        for (int x = 0; x < WK; ++x) t += slab[(x * DHP + 32 * d + tile_row(4 * q + e, h)) * 32 + l31];
-                        o[d][4 * q + e] = t;
-                    }
-                }
-    }
-    if (!live) return;
-    auto mine = [&](int q) { return WK == 1 || q == wk; };
-    if (a.splits > 1) {
-        const int64_t rt = (n * a.G + g) * a.R + row, rows = a.N * a.G * a.R;
-        float* pr = a.part + (sp * rows + rt) * a.dhs;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int c = 32 * d + 8 * q + 4 * h;
-                if (mine(q)) store4<true>(pr + c, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, a.dhs - c);
-            }
-        if (h == 0 && wk == 0) { a.part_ml[2 * (sp * rows + rt)] = m; a.part_ml[2 * (sp * rows + rt) + 1] = l; }
-        return;
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);          // no key: a zero row (and a NaN stays one)
-    T* op = static_cast<T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = 32 * d + 8 * q + 4 * h;
-            if (mine(q)) store4<VEC>(op + c, f32x4{o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv}, a.dh - c);
-        }
-    if (a.row_max && h == 0 && wk == 0) {
-        const int64_t x = (n * a.H + head) * a.Sq + i;
-        a.row_max[x] = l == 0.f ? 0.f : (NAT ? m : m * LN2);
-        a.row_sum[x] = l == 0.f ? 1.f : l;
-    }
-}
-
-// joins the splits of a row: four output columns per thread
-template <class T>
-__global__ __launch_bounds__(256) void attn_join_kernel(const Args a) {
-    constexpr bool NAT = sizeof(T) == 4;
-    const int quads = a.dhs / 4;
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = a.N * a.G * a.R;
-    if (idx >= rows * quads) return;
-    const int64_t rt = idx / quads;
-    const int c = (int)(idx - rt * quads) * 4;
-    float M = NEVER;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + rt)]);
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float ms = a.part_ml[2 * (s * rows + rt)], f = __builtin_amdgcn_exp2f(NAT ? (ms - M) * LOG2E : ms - M);
-        l += a.part_ml[2 * (s * rows + rt) + 1] * f;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (s * rows + rt) * a.dhs + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
-    }
-    const int64_t ng = rt / a.R;
-    const int row = (int)(rt - ng * a.R), hh = row / a.Sq, i = row - hh * a.Sq;
-    const int64_t n = ng / a.G, head = (ng - n * a.G) * a.rep + hh;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= inv;
-    store4<false>(static_cast<T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h + c, o, a.dh - c);
-    if (a.row_max && c == 0) {
-        const int64_t x = (n * a.H + head) * a.Sq + i;
-        a.row_max[x] = l == 0.f ? 0.f : (NAT ? M : M * LN2);
-        a.row_sum[x] = l == 0.f ? 1.f : l;
-    }
-}
-
-// ---------------------------------------------------------------- host
 Args make_args(const AttnProblem& p) {
     Args a{};
     a.q = p.q; a.k = p.k; a.v = p.v; a.mask = p.key_mask;
@@ -304,85 +12,100 @@ Args make_args(const AttnProblem& p) {
     a.N = p.N; a.Sq = p.Sq; a.Sk = p.Sk; a.H = p.H; a.G = p.G; a.rep = p.H / p.G; a.dh = p.dh; a.dhs = (p.dh + 3) / 4 * 4;
     a.R = a.rep * p.Sq;
     a.causal = p.causal; a.additive = p.additive; a.scale = p.scale; a.fill = p.dc.mask_fill;
-    a.drop = p.dc.p > 0.f; a.keep = a.drop ? 1.f / (1.f - p.dc.p) : 1.f;
+    a.keep = p.dc.p > 0.f ? 1.f / (1.f - p.dc.p) : 1.f;
     a.thr = drop_threshold(p.dc.p); a.site = p.dc.site; a.seed = p.dc.seed;
     a.splits = 1;
     return a;
 }
-bool aligned16(const void* ptr, const AttnStrides& st, int dh, size_t elem) {
-    const int64_t e = 16 / (int64_t)elem;
-    return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && dh % e == 0 && st.n % e == 0 && st.s % e == 0 && st.h % e == 0;
-}
-bool all_aligned(const AttnProblem& p) {
+static bool all_aligned(const AttnProblem& p) {
     const size_t e = p.bf16 ? 2 : 4;
-    return aligned16(p.q, p.sq, p.dh, e) && aligned16(p.k, p.sk, p.dh, e) && aligned16(p.v, p.sv, p.dh, e);
+    return aligned16(p.q, p.sq, p.dh, e, 128) && aligned16(p.k, p.sk, p.dh, e, 128) && aligned16(p.v, p.sv, p.dh, e, 128);
 }
-// workgroups that leave the chip half empty (fewer than 2 per CU) split `length` further, down to 256 of it each
-Split split_axis(int64_t blocks, int length, int unit) {
+// workgroups that do not reach every CU split `length` further, to about two per CU and down to 256 of it each
+static Split split_axis(int64_t blocks, int length, int unit) {
     Split s{1, length};
-    if (blocks <= 0 || blocks >= 512 || length <= 512) return s;
+    if (blocks <= 0 || blocks >= 256 || length <= 512) return s;
     const int64_t want = std::min<int64_t>((512 + blocks - 1) / blocks, length / 256);
     s.per = (int)((((int64_t)length + want - 1) / want + unit - 1) / unit * unit);
     s.splits = (length + s.per - 1) / s.per;
     return s;
 }
+// causal rows go by blocks of one query head, so that the blocks with most keys can come first
+static int head_blocks(const AttnProblem& p, int rows) { return p.causal && p.Sq >= rows ? cdiv(p.Sq, rows) : 0; }
 
-struct FwdPlan { int wk; int nblk; Split sp; size_t ws; };
+struct FwdPlan { int wk, nblk, head_blocks; Split sp; size_t ws; };
 static FwdPlan plan_fwd(const AttnProblem& p) {
     FwdPlan f;
     const int64_t R = (int64_t)(p.H / p.G) * p.Sq;
     f.wk = R <= 32 ? 4 : 1;
-    f.nblk = cdiv(R, 32 * (4 / f.wk));
+    f.head_blocks = f.wk == 1 ? head_blocks(p, 128) : 0;
+    f.nblk = f.head_blocks ? p.H / p.G * f.head_blocks : cdiv(R, 32 * (4 / f.wk));
     f.sp = split_axis(p.N * p.G * f.nblk, p.Sk, 128);
     const size_t rows = (size_t)(p.N * p.G * R);
     f.ws = f.sp.splits > 1 ? f.sp.splits * rows * (size_t)((p.dh + 3) / 4 * 4 + 2) * 4 : 0;
     return f;
 }
+static BwdPlan plan_bwd(const AttnProblem& p) {
+    BwdPlan f;
+    const int64_t R = (int64_t)(p.H / p.G) * p.Sq;
+    f.wk = R <= 32 ? 4 : 1;
+    f.head_blocks = f.wk == 1 ? head_blocks(p, 128) : 0;
+    f.nblk_q = f.head_blocks ? p.H / p.G * f.head_blocks : cdiv(R, 32 * (4 / f.wk));
+    f.nblk_k = cdiv(p.Sk, 128);
+    f.q = split_axis(p.N * p.G * f.nblk_q, p.Sk, 128);
+    f.kv = split_axis(p.N * p.G * f.nblk_k, (int)R, 64);
+    const size_t row = (size_t)((p.dh + 3) / 4 * 4) * 4;
+    const size_t wq = f.q.splits > 1 ? f.q.splits * (size_t)(p.N * p.G * R) * row : 0;
+    const size_t wk = f.kv.splits > 1 ? 2 * f.kv.splits * (size_t)(p.N * p.G * p.Sk) * row : 0;
+    f.ws = std::max(wq, wk);                     // the two passes run one after the other
+    return f;
+}
 
-template <class T, int DHP, bool VEC, int WK>
-static int launch_fwd(const Args& a, unsigned grid, hipStream_t s) {
-    constexpr size_t bytes = FwdCfg<T, DHP, WK>::BYTES;
-    if (bytes > 64 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_fwd_kernel<T, DHP, VEC, WK>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DHP, VEC, WK>), dim3(grid), dim3(256), bytes, s, a);
-    return check_launch("attention_fwd");
-}
-template <class T, bool VEC, int WK>
-static int pick_fwd(const Args& a, unsigned grid, hipStream_t s) {
-    if (a.dh <= 32) return launch_fwd<T, 32, VEC, WK>(a, grid, s);
-    if (a.dh <= 64) return launch_fwd<T, 64, VEC, WK>(a, grid, s);
-    return launch_fwd<T, 128, VEC, WK>(a, grid, s);
-}
-template <class T>
-static int run_fwd(const Args& a, bool vec, int wk, unsigned grid, hipStream_t s) {
-    int rc = wk == 4 ? (vec ? pick_fwd<T, true, 4>(a, grid, s) : pick_fwd<T, false, 4>(a, grid, s))
-                     : (vec ? pick_fwd<T, true, 1>(a, grid, s) : pick_fwd<T, false, 1>(a, grid, s));
-    if (rc != NR_OK || a.splits == 1) return rc;
-    const int64_t threads = a.N * a.G * a.R * (a.dhs / 4);
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a);
-    return check_launch("attention_fwd join");
-}
+extern template int run_fwd<float>(const Args&, bool, bool, int, unsigned, hipStream_t);
+extern template int run_fwd<__bf16>(const Args&, bool, bool, int, unsigned, hipStream_t);
+extern template int run_bwd<float>(Args, const BwdPlan&, bool, bool, bool, hipStream_t);
+extern template int run_bwd<__bf16>(Args, const BwdPlan&, bool, bool, bool, hipStream_t);
 
 }  // namespace al
 
 size_t attn_long_fwd_ws_bytes(const AttnProblem& p) { return al::plan_fwd(p).ws; }
 
 int attn_long_fwd(const AttnProblem& p, const AttnOut& o, void* ws, size_t ws_bytes, hipStream_t s) {
-    const al::FwdPlan f = al::plan_fwd(p);
     if (p.N == 0 || p.Sq == 0) return NR_OK;
+    const al::FwdPlan f = al::plan_fwd(p);
     al::Args a = al::make_args(p);
     a.out = o.out; a.so = o.so; a.row_max = o.row_max; a.row_sum = o.row_sum;
-    a.nblk_r = f.nblk; a.splits = f.sp.splits; a.per_split = f.sp.per;
+    a.nblk = f.nblk; a.head_blocks = f.head_blocks; a.splits = f.sp.splits; a.per_split = f.sp.per;
     if (f.ws && (!ws || ws_bytes < f.ws)) {      // without room for the joins the keys stay with one workgroup
         a.splits = 1; a.per_split = p.Sk;
     } else if (f.ws) {
         a.part = static_cast<float*>(ws);
         a.part_ml = a.part + (size_t)a.splits * (p.N * p.G * a.R) * a.dhs;
     }
-    const int64_t grid = p.N * p.G * (int64_t)a.nblk_r * a.splits;
+    const int64_t grid = p.N * p.G * (int64_t)a.nblk * a.splits;
     NR_UNSUPPORTED(grid > 0x7fffffff, "attention_fwd: %lld workgroups", (long long)grid);
-    const bool vec = al::all_aligned(p) && al::aligned16(o.out, o.so, p.dh, p.bf16 ? 2 : 4);
-    return p.bf16 ? al::run_fwd<__bf16>(a, vec, f.wk, (unsigned)grid, s) : al::run_fwd<float>(a, vec, f.wk, (unsigned)grid, s);
+    const bool vec = al::all_aligned(p) && al::aligned16(o.out, o.so, p.dh, p.bf16 ? 2 : 4, 128), drop = p.dc.p > 0.f;
+    return p.bf16 ? al::run_fwd<__bf16>(a, vec, drop, f.wk, (unsigned)grid, s) : al::run_fwd<float>(a, vec, drop, f.wk, (unsigned)grid, s);
+}
+
+size_t attn_long_bwd_ws_bytes(const AttnProblem& p) { return al::plan_bwd(p).ws; }
+
+int attn_long_bwd(const AttnProblem& p, const AttnGrad& g, void* ws, size_t ws_bytes, hipStream_t s) {
+    if (p.N == 0 || p.Sq == 0 || p.Sk == 0) return NR_OK;
+    const al::BwdPlan f = al::plan_bwd(p);
+    const int64_t grid = p.N * p.G * std::max<int64_t>((int64_t)f.nblk_k * f.kv.splits, (int64_t)f.nblk_q * f.q.splits);
+    const int64_t rows = p.N * p.Sq * p.H;
+    NR_UNSUPPORTED(grid > 0x7fffffff || rows > ((int64_t)1 << 34), "attention_bwd: %lld workgroups, %lld rows", (long long)grid, (long long)rows);
+    al::Args a = al::make_args(p);
+    a.out = const_cast<void*>(g.out); a.so = g.so; a.dout = g.dout; a.sdo = g.sdo;
+    a.row_max = const_cast<float*>(g.row_max); a.row_sum = const_cast<float*>(g.row_sum);
+    a.delta = g.delta; a.sd = g.sd;
+    a.dq = g.dq; a.dk = g.dk; a.dv = g.dv; a.sdq = g.sdq; a.sdk = g.sdk; a.sdv = g.sdv;
+    a.part = static_cast<float*>(ws);
+    const size_t e = p.bf16 ? 2 : 4;
+    const bool vec = al::all_aligned(p) && al::aligned16(g.dout, g.sdo, p.dh, e, 128) && al::aligned16(g.dq, g.sdq, p.dh, e, 128);
+    const bool room = !f.ws || (ws && ws_bytes >= f.ws), drop = p.dc.p > 0.f;      // without room for the partial sums nothing is split
+    return p.bf16 ? al::run_bwd<__bf16>(a, f, vec, drop, room, s) : al::run_bwd<float>(a, f, vec, drop, room, s);
 }
 
 }  // namespace nr

@@ -1,4 +1,4 @@
-// device pieces shared by the forward and backward kernels of attention_long*.hip
+// device pieces shared by the forward and backward kernels of attention of any length (attention_long_fwd.h, attention_long_bwd.h)
 #pragma once
 #include "attention_long.h"
 #include "mma.h"
@@ -16,7 +16,7 @@ struct Args {
     int64_t N;
     int Sq, Sk, H, G, rep, dh, dhs;             // rep = H / G; dhs = dh rounded up to 4 (row length of the partial results)
     int R;                                      // rep * Sq: the rows of one key head (query head major)
-    int causal, additive, drop;
+    int causal, additive;
     float scale, fill, keep;                    // keep = 1 / (1 - p)
     uint32_t thr, site;
     uint64_t seed;
@@ -29,21 +29,36 @@ struct Args {
     void *dq, *dk, *dv; AttnStrides sdq, sdk, sdv;
     // split of the long axis
     float* part; float* part_ml;
-    int nblk_r;                                 // row (dKV: key) blocks of one key head
+    int nblk;                                   // row (dKV: key) blocks of one key head
+    int head_blocks;                            // > 0: row blocks of one query head, none of which reaches into the next head
     int splits, per_split;
 };
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NEVER = -1e30f;                 // running maximum before the first key: finite, so exp2(-inf - NEVER) = 0 and no inf - inf
 
-// neighbouring workgroups go to different XCDs; this order gives each XCD a contiguous run of the logical ones, so that blocks
-// which read the same key head share an L2
-__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
-    const uint32_t x = b & 7, q = n >> 3, rem = n & 7;
-    return x * q + (x < rem ? x : rem) + (b >> 3);
+// Neighbouring workgroups go to different XCDs, each with its own L2.  Key heads are dealt to the XCDs, so that the workgroups of one
+// head share an L2 and sequences of different lengths still spread over the chip; what is left of a multiple of 8 heads is spread
+// block by block.  (Contiguous runs of blocks per XCD, which this replaced, left XCDs idle whenever neighbouring sequences were
+// short: 32 x 512 with lengths 128 .. 512 took as long as 32 x 512 without padding.)
+struct Slot { int head, w; };                   // key head (n * G + g), block of that head
+__device__ __forceinline__ Slot deal(uint32_t b, uint32_t heads, uint32_t per_head) {
+    const uint32_t full = heads & ~7u;
+    if (b < full * per_head) {
+        const uint32_t slot = b >> 3, q = slot / per_head;
+        return Slot{(int)(q * 8 + (b & 7)), (int)(slot - q * per_head)};
+    }
+    b -= full * per_head;
+    const uint32_t left = heads - full, w = b / left;
+    return Slot{(int)(full + b - w * left), (int)w};
 }
-// the causal rows' work grows with the row: heavy and light blocks alternate within a head
-__device__ __forceinline__ int heavy_light(int i, int n) { return (i & 1) ? (i >> 1) : n - 1 - (i >> 1); }
+// rows [r0, rend) of row block w: with causal order the blocks with most keys come first, one query head per block
+struct Rows { int r0, rend; };
+__device__ __forceinline__ Rows row_block(const Args& a, int w, int rows) {
+    if (!a.head_blocks) return Rows{w * rows, a.R};
+    const int p = w / a.rep, hh = w - p * a.rep;
+    return Rows{hh * a.Sq + (a.head_blocks - 1 - p) * rows, (hh + 1) * a.Sq};
+}
 
 // keep bits of the probabilities (row_linear, j) .. (row_linear, j + 3): element index row_linear * Sk + j of the library's stream
 __device__ __forceinline__ uint32_t keep4(const Args& a, uint64_t idx) {
@@ -63,70 +78,106 @@ __device__ __forceinline__ uint32_t keep4(const Args& a, uint64_t idx) {
     return m;
 }
 
-// A [ROWS x DHP] tile on its way from global memory into LDS, 16 bytes per piece: `load` only issues the loads, `store` waits.
-// row_ptr(row) gives the row's address, or NULL for a row that has to read as zero.
-template <class T, int DHP, int ROWS, bool VEC>
+// Rows [0, rows) of a [ROWS x DHP] tile on their way from global memory into LDS, 16 bytes per piece: `load` only issues the loads,
+// `store` waits.  Rows past `rows` and columns past dh read as zero.  VEC: buffer loads whose bounds check does that, with one
+// 32-bit offset per thread (the host checks that a tile's offsets fit); otherwise element by element.
+template <class T, int DHP, int ROWS, bool VEC, int NT = 256>
 struct Stage {
-    static constexpr int E = Ty<T>::E, PITCH = DHP + Ty<T>::PAD, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / 256;
-    static_assert(ROWS * PER_ROW % 256 == 0, "whole pieces per thread");
+    static constexpr int E = Ty<T>::E, PITCH = DHP + Ty<T>::PAD, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / NT, STEP = NT / PER_ROW;
+    static_assert(ROWS * PER_ROW % NT == 0 && NT % PER_ROW == 0, "whole pieces per thread, whole rows per pass");
     u32x4 r[NCH];
-    template <class F> __device__ __forceinline__ void load(int tid, int dh, F row_ptr) {
-#pragma unroll
-        for (int u = 0; u < NCH; ++u) {
-            const int c = tid + 256 * u, row = c / PER_ROW, col = (c % PER_ROW) * E;
-            const T* p = row_ptr(row);
-            r[u] = load16<T, VEC>(p + col, p ? dh - col : 0);
+    int row, col;
+    uint32_t voff, step;
+    __device__ __forceinline__ void setup(int tid, int64_t stride, int dh) {
+        row = tid / PER_ROW;
+        col = (tid % PER_ROW) * E;
+        if (VEC) {
+            voff = col < dh ? (uint32_t)(row * (int)stride + col) * (uint32_t)sizeof(T) : 0x80000000u;
+            step = STEP * (uint32_t)stride * (uint32_t)sizeof(T);
         }
     }
-    template <class F> __device__ __forceinline__ void store(int tid, T* lds, F keep) {
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dh) {
+        if (VEC) {
+            const uint64_t bytes = rows > 0 ? ((uint64_t)(rows - 1) * (uint64_t)stride + dh) * sizeof(T) : 0;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(base), 0, (int)(bytes < 0x7fffffffu ? bytes : 0x7fffffffu), 0x00020000);
 #pragma unroll
-        for (int u = 0; u < NCH; ++u) {
-            const int c = tid + 256 * u, row = c / PER_ROW, col = (c % PER_ROW) * E;
-            *reinterpret_cast<u32x4*>(lds + row * PITCH + col) = keep(row) ? r[u] : u32x4{0, 0, 0, 0};
+            for (int u = 0; u < NCH; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(voff + u * step), 0, 0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NCH; ++u)
+                r[u] = load16<T, false>(base + (int64_t)(row + STEP * u) * stride + col, row + STEP * u < rows ? dh - col : 0);
         }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int u = 0; u < NCH; ++u) *reinterpret_cast<u32x4*>(lds + (row + STEP * u) * PITCH + col) = r[u];
+    }
+    template <class F> __device__ __forceinline__ void store_if(T* lds, F keep) const {
+#pragma unroll
+        for (int u = 0; u < NCH; ++u)
+            *reinterpret_cast<u32x4*>(lds + (row + STEP * u) * PITCH + col) = keep(row + STEP * u) ? r[u] : u32x4{0, 0, 0, 0};
     }
 };
 
-// presence bits of the WORDS * 64 keys from j on.  load() issues, bits() waits; every wave holds all of them
-template <int WORDS>
+// Which keys are there, a bit each, for up to SPAN keys from `from` on: read once, kept in LDS.  Without a mask the bits follow from
+// the end alone.
+constexpr int SPAN = 8192;
 struct KeyBits {
-    int64_t m[WORDS];
-    __device__ __forceinline__ void load(const int64_t* mask, int j, int end, int lane) {
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-            const int key = j + 64 * w + lane;
-            m[w] = mask ? (key < end ? mask[key] : 0) : (key < end);
+    uint64_t* words;                            // [SPAN / 64] in LDS
+    bool masked;
+    int from, end;                              // keys [from, end)
+    // all threads; returns the end of the last key that is there (>= from)
+    __device__ __forceinline__ int fill(const int64_t* mask, int lane, int wave) {
+        const int n = (end - from + 63) >> 6;
+#pragma unroll 4
+        for (int x = wave; x < n; x += 4) {
+            const int key = from + 64 * x + lane;
+            const uint64_t b = __ballot(key < end && mask[key] != 0);
+            if (lane == 0) words[x] = b;
         }
+        __syncthreads();
+        const uint64_t lo = __ballot(lane < n && words[lane] != 0), hi = __ballot(64 + lane < n && words[64 + lane] != 0);
+        if (!(lo | hi)) return from;
+        const int top = hi ? 127 - __builtin_clzll(hi) : 63 - __builtin_clzll(lo);
+        return from + 64 * top + 64 - __builtin_clzll(words[top]);
     }
-    __device__ __forceinline__ uint64_t bits(int w) const { return __ballot(m[w] != 0); }
+    __device__ __forceinline__ uint64_t range(int j) const {
+        const int left = end - j;
+        return left >= 64 ? ~0ull : (left > 0 ? (1ull << left) - 1 : 0ull);
+    }
+    // 64 keys from j (a multiple of 32 past `from`) on; wave-uniform
+    __device__ __forceinline__ uint64_t at(int j) const {
+        if (!masked) return range(j);
+        if (j >= end) return 0;
+        const int x = (j - from) >> 6;
+        const uint64_t w = words[x];
+        const uint64_t u = (uint64_t)__builtin_amdgcn_readfirstlane((int)(w >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)w);
+        return ((j - from) & 32) ? u >> 32 : u;
+    }
 };
 
-// the end of the keys a block has to read: `end`, less whole runs of 256 absent keys at the end of [begin, end)
-__device__ __forceinline__ int present_end(const int64_t* mask, int begin, int end, int tid) {
-    while (end > begin) {
-        const int j = end - 256 + tid;
-        const int there = j >= begin && mask[j] != 0;
-        if (__syncthreads_or(there)) break;
-        end -= 256;
-    }
-    return end > begin ? end : begin;
-}
-
-// [sub] x 16 scores of this lane's row -> the same with what the row must not see taken out.  key0: the key of register 0's row 0
+// scores of this lane's row, 16 keys of 32 from key0 on: what the row must not see becomes -inf
 __device__ __forceinline__ void hide(f32x16& x, uint32_t bits, int key0, int lim, int h) {
+    if (lim - key0 < 31) bits = lim < key0 ? 0 : bits & ((2u << (lim - key0)) - 1);
+    bits >>= 4 * h;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int t = tile_row(r, h);
-        if (!((bits >> t) & 1) || key0 + t > lim) x[r] = -INFINITY;
-    }
+    for (int r = 0; r < 16; ++r)
+        if (!((bits >> tile_row(r, 0)) & 1)) x[r] = -INFINITY;
 }
 
 // host side
+// 16-byte loads and stores: the address and every stride a multiple of 16 bytes; `tile` rows of it within a 32-bit offset
+inline bool aligned16(const void* ptr, const AttnStrides& st, int dh, size_t elem, int tile) {
+    const int64_t e = 16 / (int64_t)elem;
+    return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && dh % e == 0 && st.n % e == 0 && st.s % e == 0 && st.h % e == 0 &&
+           st.s >= 0 && st.s < ((int64_t)1 << 31) / (tile * (int64_t)elem);
+}
 Args make_args(const AttnProblem& p);
-bool aligned16(const void* ptr, const AttnStrides& st, int dh, size_t elem);
-bool all_aligned(const AttnProblem& p);
+template <class T> int run_fwd(const Args& a, bool vec, bool drop, int wk, unsigned grid, hipStream_t s);
 struct Split { int splits, per; };
-Split split_axis(int64_t blocks, int length, int unit);
+struct BwdPlan { int wk, nblk_q, nblk_k, head_blocks; Split q, kv; size_t ws; };
+template <class T> int run_bwd(Args a, const BwdPlan& f, bool vec, bool drop, bool room, hipStream_t s);
 
 }  // namespace al
 }  // namespace nr

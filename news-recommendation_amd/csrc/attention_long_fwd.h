@@ -1,0 +1,352 @@
+// Softmax attention of any length: forward kernels (instantiated by attention_long_fwd_{f32,bf16}.hip).
+//
+//   o_i = sum_j p_ij v_j,   p_ij = exp(x_ij - max_j x_ij) / sum_j exp(..),   x_ij = scale * q_i . k_j
+//
+// over the keys j that are there (key mask) and, causal, not behind the query (j <= i + Sk - Sq).  One pass over the keys with
+// the running maximum m and sum l of every row: a new tile's maximum m' rescales what was summed so far by exp(m - m').
+//
+// Tiling.  A workgroup of four waves takes 128 rows of one key head and walks the keys in tiles staged through LDS; a wave owns
+// 32 rows.  The query heads that share a key head are laid one below the other (row r = query head r / Sq, position r % Sq), so
+// K and V are read once for all of them.  A wave forms S^T = K Q^T (row = key, column = query): a lane then holds 16 scores of
+// ONE row per 32 keys, the softmax needs one exchange (the other lane half), and the probabilities are, register by register, the
+// B operand of O^T += V^T P^T (mma.h, "tile" order) - they never pass through LDS.
+// With at most 32 rows (a few candidates over a long history) the four waves take a quarter of every tile's keys each instead
+// (WK = 4) and meet at the end through LDS; when the workgroups do not fill the chip the keys are also split over workgroups
+// and joined by attn_join_kernel.
+//
+// Rounding: scores, maximum, sum and output are fp32; bf16 inputs round the probabilities to bf16 (the matrix instruction's
+// operand), half a step each, against a sum taken in fp32 from the unrounded ones.
+#pragma once
+#include "attention_long_dev.h"
+
+namespace nr {
+namespace al {
+
+template <class T, int DHP, int WK> struct FwdCfg {
+    static constexpr int KSUB = (sizeof(T) == 2 && WK == 1) ? 2 : 1;     // 32-key pieces of a tile per wave
+    static constexpr int KT = 32 * KSUB * WK;
+    static constexpr int PITCH = DHP + Ty<T>::PAD;
+    static constexpr int NBUF = (sizeof(T) == 4 && DHP == 128 && WK == 4) ? 1 : 2;       // two stages where 160 KB hold them
+    static constexpr size_t TILES = (size_t)NBUF * 2 * KT * PITCH * sizeof(T);
+    static constexpr size_t JOIN = WK > 1 ? (size_t)(WK * DHP * 32 + 2 * WK * 32) * 4 : 0;
+    static constexpr size_t BITS = TILES > JOIN ? TILES : JOIN;          // offset of the key bits
+    static constexpr size_t BYTES = BITS + SPAN / 8;
+    static constexpr int WAVES = BYTES <= 80 * 1024 ? 2 : 1;             // per SIMD: registers for two where the LDS holds two
+};
+
+template <class T, int DHP, bool VEC, int WK, bool DROP>
+__global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_kernel(const Args a) {
+    typedef FwdCfg<T, DHP, WK> C;
+    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, PITCH = C::PITCH, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
+    constexpr bool NAT = sizeof(T) == 4;         // fp32: exp(x - m) with the difference formed first (the mask's -1e5 would cost
+                                                 // a product's rounding); bf16: one fma per score in units of log 2
+    // the maximum may lag behind by this much before the sums are rescaled (bf16: probabilities up to 2^8, no precision is lost
+    // in a floating format; the rescaling of every row's sums becomes rare)
+    constexpr float SLACK = NAT ? 0.f : 8.f;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* Ks = reinterpret_cast<T*>(smem);
+    T* Vs = Ks + C::NBUF * KT * PITCH;
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wq = w / WK, wk = w % WK;
+
+    const Slot slot = deal(blockIdx.x, (uint32_t)(a.N * a.G), a.nblk * a.splits);
+    const int64_t n = slot.head / a.G;
+    const int g = slot.head - (int)n * a.G, rb = slot.w / a.splits, sp = slot.w - rb * a.splits;
+    const Rows rows = row_block(a, rb, 32 * WQ);
+
+    // this lane's row
+    const int row = rows.r0 + 32 * wq + l31;
+    const bool live = row < rows.rend;
+    const int hh = live ? row / a.Sq : 0, i = live ? row - hh * a.Sq : 0, head = g * a.rep + hh;
+    const int lim = a.causal ? i + a.Sk - a.Sq : 0x7fffffff;             // last key of the row
+    int lim_min = live ? lim : 0x7fffffff;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o, 64));
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    typename Ty<T>::Frag qf[KS];
+    const T* qp = static_cast<const T*>(a.q) + n * a.sq.n + i * a.sq.s + head * a.sq.h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<VEC>(qp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
+
+    // keys of this block
+    int begin = sp * a.per_split, stop = min(a.Sk, begin + a.per_split);
+    if (a.causal) {
+        const int last = min(rows.r0 + 32 * WQ, rows.rend) - 1;
+        const int imax = rows.r0 / a.Sq == last / a.Sq ? last % a.Sq : a.Sq - 1;
+        stop = min(stop, imax + a.Sk - a.Sq + 1);
+    }
+    const int64_t* mask = a.mask ? a.mask + n * a.Sk : nullptr;
+    const bool cut = mask && !a.additive;        // keys that are not there need not be read
+    const T* kp = static_cast<const T*>(a.k) + n * a.sk.n + g * a.sk.h;
+    const T* vp = static_cast<const T*>(a.v) + n * a.sv.n + g * a.sv.h;
+
+    const float scale2 = a.scale * LOG2E;
+    float m = NEVER, l = 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = zero16();
+
+    Stage<T, DHP, KT, VEC> sk, sv;
+    sk.setup(tid, a.sk.s, a.dh);
+    sv.setup(tid, a.sv.s, a.dh);
+    KeyBits kb;
+    kb.words = reinterpret_cast<uint64_t*>(smem + C::BITS);
+    kb.masked = mask != nullptr;
+    for (; begin < stop; begin += SPAN) {        // (one turn without a mask)
+        int end = stop;
+        kb.from = begin;
+        kb.end = stop;
+        if (mask) {
+            kb.end = end = min(stop, begin + SPAN);
+            const int there = kb.fill(mask, lane, w);
+            if (cut) kb.end = end = there;
+        }
+        auto fetch = [&](int j) {
+            sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
+            sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
+        };
+        auto put = [&](int buf, int j) {
+            // an absent key's row reads as zero: whatever its memory holds (a NaN as well) must not reach 0 * v
+            uint64_t bits[WORDS];
+            bool all = true;
+#pragma unroll
+            for (int x = 0; x < WORDS; ++x) {
+                bits[x] = cut ? kb.at(j + 64 * x) : ~0ull;
+                all = all && (KT < 64 ? (uint32_t)bits[x] == ~0u : bits[x] == ~0ull);
+            }
+            if (all) {
+                sk.store(Ks + buf * KT * PITCH);
+                sv.store(Vs + buf * KT * PITCH);
+            } else {
+                auto keep = [&](int r) { return (bits[WORDS > 1 ? r >> 6 : 0] >> (r & 63)) & 1; };
+                sk.store_if(Ks + buf * KT * PITCH, keep);
+                sv.store_if(Vs + buf * KT * PITCH, keep);
+            }
+        };
+        const int tiles = (end - begin + KT - 1) / KT;
+        if (tiles > 0) { fetch(begin); put(0, begin); }
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
+            fetch(j0 + KT);                      // (past the end: zeros, no memory is read)
+            const T* Kt = Ks + buf * KT * PITCH;
+            const T* Vt = Vs + buf * KT * PITCH;
+            const int kw = j0 + 32 * wk * KSUB;                          // first key of this wave's piece
+            const uint64_t mine = kb.at(kw);
+            uint32_t sub[KSUB], any = 0, all = ~0u;
+#pragma unroll
+            for (int s = 0; s < KSUB; ++s) {
+                sub[s] = (uint32_t)(mine >> (32 * s));
+                any |= sub[s]; all &= sub[s];
+            }
+            if (any || (a.additive && kw < end)) {
+                f32x16 x[KSUB];
+#pragma unroll
+                for (int s = 0; s < KSUB; ++s) {
+                    x[s] = zero16();
+                    const T* kr = Kt + (32 * (wk * KSUB + s) + l31) * PITCH + 8 * h;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) x[s] = mul(near_frag(kr + 16 * ks), qf[ks], x[s]);
+                }
+                if (NAT) {
+#pragma unroll
+                    for (int s = 0; s < KSUB; ++s) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[s][r] *= a.scale;
+                        if (a.additive) {                                // absent keys sink by `fill`; past the end there is no key
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) if (!((sub[s] >> tile_row(r, h)) & 1)) x[s][r] += a.fill;
+                            sub[s] = (uint32_t)kb.range(kw + 32 * s);
+                            all = s ? all & sub[s] : sub[s];
+                        }
+                    }
+                }
+                if (all != ~0u || kw + 32 * KSUB - 1 > lim_min)
+#pragma unroll
+                    for (int s = 0; s < KSUB; ++s) hide(x[s], sub[s], kw + 32 * s, lim, h);
+                float top = x[0][0];
+#pragma unroll
+                for (int s = 0; s < KSUB; ++s)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, x[s][r]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = NAT ? top : top * scale2;
+                if (__any(mn > m + SLACK)) {
+                    const float to = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(NAT ? (m - to) * LOG2E : m - to);
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+                    m = to;
+                }
+                float sum = 0.f;
+#pragma unroll
+                for (int s = 0; s < KSUB; ++s)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[s][r] = __builtin_amdgcn_exp2f(NAT ? (x[s][r] - m) * LOG2E : fmaf(x[s][r], scale2, -m));
+                        sum += x[s][r];
+                    }
+                l += sum;
+                if (DROP) {
+                    const uint64_t rl = ((uint64_t)(n * a.H + head) * a.Sq + i) * a.Sk;
+#pragma unroll
+                    for (int s = 0; s < KSUB; ++s)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t kp4 = keep4(a, rl + kw + 32 * s + 8 * q + 4 * h);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[s][4 * q + e] *= ((kp4 >> e) & 1) ? a.keep : 0.f;
+                        }
+                }
+#pragma unroll
+                for (int s = 0; s < KSUB; ++s)
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        const typename Ty<T>::Frag pf = tile_frag<T>(x[s], k2);
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+                            o[d] = mul(col_frag<PITCH>(Vt, 32 * (wk * KSUB + s) + 16 * k2, 32 * d, lane), pf, o[d]);
+                    }
+            }
+            if (C::NBUF == 1) __syncthreads();
+            put(C::NBUF == 2 ? 1 - buf : 0, j0 + KT);
+            __syncthreads();
+        }
+        if (!mask) break;
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    if (WK > 1) {                                // the waves' quarters of the keys meet (in wave order: the same result every time)
+        float* slab = reinterpret_cast<float*>(smem);                    // [WK][DHP][32]
+        float* ml = slab + WK * DHP * 32;                                // [2][WK][32]
+        __syncthreads();
+        if (h == 0) { ml[wk * 32 + l31] = m; ml[(WK + wk) * 32 + l31] = l; }
+        __syncthreads();
+        float M = NEVER;
+#pragma unroll
+        for (int x = 0; x < WK; ++x) M = fmaxf(M, ml[x * 32 + l31]);
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < WK; ++x)
+            sum += ml[(WK + x) * 32 + l31] * __builtin_amdgcn_exp2f(NAT ? (ml[x * 32 + l31] - M) * LOG2E : ml[x * 32 + l31] - M);
+        const float f = __builtin_amdgcn_exp2f(NAT ? (m - M) * LOG2E : m - M);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) slab[(wk * DHP + 32 * d + tile_row(r, h)) * 32 + l31] = o[d][r] * f;
+        __syncthreads();
+        m = M; l = sum;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q == wk % 4) {               // wave wk finishes registers 4 wk .. 4 wk + 3 of every tile
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float t = 0.f;
+#pragma unroll
+                        for (int x = 0; x < WK; ++x) t += slab[(x * DHP + 32 * d + tile_row(4 * q + e, h)) * 32 + l31];
+                        o[d][4 * q + e] = t;
+                    }
+                }
+    }
+    if (!live) return;
+    auto mine = [&](int q) { return WK == 1 || q == wk; };
+    if (a.splits > 1) {
+        const int64_t rt = (n * a.G + g) * a.R + row, total = a.N * a.G * a.R;
+        float* pr = a.part + (sp * total + rt) * a.dhs;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = 32 * d + 8 * q + 4 * h;
+                if (mine(q)) store4<true>(pr + c, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, a.dhs - c);
+            }
+        if (h == 0 && wk == 0) { a.part_ml[2 * (sp * total + rt)] = m; a.part_ml[2 * (sp * total + rt) + 1] = l; }
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);          // no key: a zero row (and a NaN stays one)
+    T* op = static_cast<T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = 32 * d + 8 * q + 4 * h;
+            if (mine(q)) store4<VEC>(op + c, f32x4{o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv}, a.dh - c);
+        }
+    if (a.row_max && h == 0 && wk == 0) {
+        const int64_t x = (n * a.H + head) * a.Sq + i;
+        a.row_max[x] = l == 0.f ? 0.f : (NAT ? m : m * LN2);
+        a.row_sum[x] = l == 0.f ? 1.f : l;
+    }
+}
+
+// joins the splits of a row: four output columns per thread
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const Args a) {
+    constexpr bool NAT = sizeof(T) == 4;
+    const int quads = a.dhs / 4;
+    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = a.N * a.G * a.R;
+    if (idx >= rows * quads) return;
+    const int64_t rt = idx / quads;
+    const int c = (int)(idx - rt * quads) * 4;
+    float M = NEVER;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + rt)]);
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {
+        const float ms = a.part_ml[2 * (s * rows + rt)], f = __builtin_amdgcn_exp2f(NAT ? (ms - M) * LOG2E : ms - M);
+        l += a.part_ml[2 * (s * rows + rt) + 1] * f;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (s * rows + rt) * a.dhs + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+    }
+    const int64_t ng = rt / a.R;
+    const int row = (int)(rt - ng * a.R), hh = row / a.Sq, i = row - hh * a.Sq;
+    const int64_t n = ng / a.G, head = (ng - n * a.G) * a.rep + hh;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store4<false>(static_cast<T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h + c, o, a.dh - c);
+    if (a.row_max && c == 0) {
+        const int64_t x = (n * a.H + head) * a.Sq + i;
+        a.row_max[x] = l == 0.f ? 0.f : (NAT ? M : M * LN2);
+        a.row_sum[x] = l == 0.f ? 1.f : l;
+    }
+}
+
+// ---------------------------------------------------------------- launches
+template <class T, int DHP, bool VEC, int WK, bool DROP>
+static int launch_fwd(const Args& a, unsigned grid, hipStream_t s) {
+    constexpr size_t bytes = FwdCfg<T, DHP, WK>::BYTES;
+    if (bytes > 64 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_fwd_kernel<T, DHP, VEC, WK, DROP>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DHP, VEC, WK, DROP>), dim3(grid), dim3(256), bytes, s, a);
+    return check_launch("attention_fwd");
+}
+template <class T, bool VEC, int WK, bool DROP>
+static int pick_fwd(const Args& a, unsigned grid, hipStream_t s) {
+    if (a.dh <= 32) return launch_fwd<T, 32, VEC, WK, DROP>(a, grid, s);
+    if (a.dh <= 64) return launch_fwd<T, 64, VEC, WK, DROP>(a, grid, s);
+    return launch_fwd<T, 128, VEC, WK, DROP>(a, grid, s);
+}
+template <class T, bool DROP>
+static int pick_fwd(const Args& a, bool vec, int wk, unsigned grid, hipStream_t s) {
+    return wk == 4 ? (vec ? pick_fwd<T, true, 4, DROP>(a, grid, s) : pick_fwd<T, false, 4, DROP>(a, grid, s))
+                   : (vec ? pick_fwd<T, true, 1, DROP>(a, grid, s) : pick_fwd<T, false, 1, DROP>(a, grid, s));
+}
+template <class T>
+int run_fwd(const Args& a, bool vec, bool drop, int wk, unsigned grid, hipStream_t s) {
+    int rc = drop ? pick_fwd<T, true>(a, vec, wk, grid, s) : pick_fwd<T, false>(a, vec, wk, grid, s);
+    if (rc != NR_OK || a.splits == 1) return rc;
+    const int64_t threads = a.N * a.G * a.R * (a.dhs / 4);
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a);
+    return check_launch("attention_fwd join");
+}
+
+}  // namespace al
+}  // namespace nr

@@ -97,36 +97,16 @@ template <> struct Weighed<__bf16> {
     __device__ __forceinline__ f32x16 add(const bf16x8& y, const f32x16& s) const { return mul(y, hi, mul(y, mid, mul(y, lo, s))); }
 };
 
-// a [C x D] tile on its way into LDS, D padded, NT threads
-template <class T, int D, int NT, bool VEC> struct Tile {
-    static constexpr int E = Ty<T>::E, PITCH = D + Ty<T>::PAD, PER_ROW = D / E, NCH = C * PER_ROW / NT;
-    u32x4 r[NCH];
-    __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int d, int tid) {
-#pragma unroll
-        for (int u = 0; u < NCH; ++u) {
-            const int c = tid + NT * u, row = c / PER_ROW, col = (c % PER_ROW) * E;
-            r[u] = load16<T, VEC>(p + (int64_t)row * stride + col, row < rows ? d - col : 0);
-        }
-    }
-    __device__ __forceinline__ void store(T* lds, int tid) const {
-#pragma unroll
-        for (int u = 0; u < NCH; ++u) {
-            const int c = tid + NT * u, row = c / PER_ROW, col = (c % PER_ROW) * E;
-            *reinterpret_cast<u32x4*>(lds + row * PITCH + col) = r[u];
-        }
-    }
-};
-
 // where a workgroup stands: job, head, segment
 struct Place {
     int job, seg, h, s0, s1, send, nc;
     int64_t n, nh;
     float a2;
     __device__ __forceinline__ Place(const Args& a) {
-        uint32_t b = al::xcd_order(blockIdx.x, gridDim.x);
-        job = b % a.jobs; b /= a.jobs;
-        seg = b % a.G; b /= a.G;
-        nh = b;
+        const al::Slot slot = al::deal(blockIdx.x, (uint32_t)(a.N * a.H), a.G * a.jobs);
+        nh = slot.head;
+        seg = slot.w / a.jobs;
+        job = slot.w - seg * a.jobs;
         n = nh / a.H;
         h = (int)(nh - n * a.H);
         a2 = a.log_decay[h] * al::LOG2E;
@@ -157,20 +137,22 @@ __global__ __launch_bounds__(2 * DB) void lin_state_kernel(const Args a) {
     f32x16 S[AT];
 #pragma unroll
     for (int t = 0; t < AT; ++t) S[t] = zero16();
-    Tile<T, DA, NT, VEC> ty;
-    Tile<T, DB, NT, VEC> tz;
+    al::Stage<T, DA, C, VEC, NT> ty;
+    al::Stage<T, DB, C, VEC, NT> tz;
+    ty.setup(tid, J.sy.s, J.da);
+    tz.setup(tid, J.sz.s, J.db);
     auto fetch = [&](int c) {
         const int t0 = at.s0 + C * c;
-        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da, tid);
-        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db, tid);
+        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da);
+        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db);
     };
     if (at.nc) fetch(J.rev ? at.nc - 1 : 0);
     int had = -1;
     for (int t = 0; t < at.nc; ++t) {
         const int c = J.rev ? at.nc - 1 - t : t, m = min(C, at.s1 - at.s0 - C * c);
         __syncthreads();
-        ty.store(Ys, tid);
-        tz.store(Zs, tid);
+        ty.store(Ys);
+        tz.store(Zs);
         if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid, m, J.rev, J.umul);
         had = m;
         __syncthreads();
@@ -261,22 +243,25 @@ __global__ __launch_bounds__(2 * DB) void lin_out_kernel(const Args a) {
         near[r] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
         far[r] = J.amul * power(at.a2, d + 32);
     }
-    Tile<T, DA, NT, VEC> tx, ty;
-    Tile<T, DB, NT, VEC> tz;
+    al::Stage<T, DA, C, VEC, NT> tx, ty;
+    al::Stage<T, DB, C, VEC, NT> tz;
+    tx.setup(tid, J.sx.s, J.da);
+    ty.setup(tid, J.sy.s, J.da);
+    tz.setup(tid, J.sz.s, J.db);
     auto fetch = [&](int c) {
         const int t0 = at.s0 + C * c;
-        tx.load(xp + t0 * J.sx.s, J.sx.s, at.s1 - t0, J.da, tid);
-        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da, tid);
-        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db, tid);
+        tx.load(xp + t0 * J.sx.s, J.sx.s, at.s1 - t0, J.da);
+        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da);
+        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db);
     };
     if (at.nc) fetch(rev ? at.nc - 1 : 0);
     int had = -1;
     for (int t = 0; t < at.nc; ++t) {
         const int c = rev ? at.nc - 1 - t : t, t0 = at.s0 + C * c, m = min(C, at.s1 - t0);
         __syncthreads();
-        tx.store(Xs, tid);
-        ty.store(Ys, tid);
-        tz.store(Zs, tid);
+        tx.store(Xs);
+        ty.store(Ys);
+        tz.store(Zs);
         if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid, m, rev, J.umul);
         had = m;
         __syncthreads();
@@ -435,7 +420,7 @@ static int run(const Args& a, bool bf16, hipStream_t s) {
     bool vec = true;
     for (int j = 0; j < a.jobs; ++j) {
         const Job& J = a.job[j];
-        vec = vec && al::aligned16(J.x, J.sx, J.da, e) && al::aligned16(J.y, J.sy, J.da, e) && al::aligned16(J.z, J.sz, J.db, e) && al::aligned16(J.o, J.so, J.db, e);
+        vec = vec && al::aligned16(J.x, J.sx, J.da, e, C) && al::aligned16(J.y, J.sy, J.da, e, C) && al::aligned16(J.z, J.sz, J.db, e, C) && al::aligned16(J.o, J.so, J.db, e, C);
     }
     return bf16 ? (vec ? pick_a<__bf16, true>(a, s) : pick_a<__bf16, false>(a, s)) : (vec ? pick_a<float, true>(a, s) : pick_a<float, false>(a, s));
 }
