@@ -2,7 +2,7 @@
 //
 //   S_t = w S_{t-1} + k_t v_t^T,  o_t = scale * q_t S_t   (w = e^{log_decay[h]}, S_t [dk,dv])
 //
-// A chunk of 64 tokens that starts from state S gives, with i, j positions in the chunk and m its token count,
+// A chunk of 32 tokens that starts from state S gives, with i, j positions in the chunk and m its token count,
 //   o_i = scale * ( sum_{j <= i} w^{i-j} (q_i . k_j) v_j  +  w^{i+1} q_i S ),     S' = w^m S + sum_i w^{m-1-i} k_i v_i^T
 // so everything is a matrix product; the powers are of exponents >= 0 (no overflow however fast a head forgets).
 //
@@ -32,7 +32,8 @@ namespace lin {
 
 using namespace mma;
 
-constexpr int C = 64;                            // tokens per chunk
+constexpr int UNIT = 64;                         // segments are multiples of this many tokens
+template <class T> constexpr int TILE = sizeof(T) == 2 ? 64 : 32;        // tokens per LDS tile: two chunks of bf16, one of fp32
 
 struct Job {
     const void *x, *y, *z;
@@ -46,7 +47,7 @@ struct Job {
 };
 struct Args {
     Job job[3];
-    int jobs, G, per;                            // segments of `per` tokens (a multiple of C)
+    int jobs, G, per;                            // segments of `per` tokens (a multiple of UNIT)
     int64_t N;
     int S, H;
     const float* log_decay;
@@ -68,11 +69,12 @@ __device__ __forceinline__ f32x8 spread_frag(const float* p) {
     const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 8);
     return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-// what a chunk adds to the state: S += y^T (w z), k-step kb of it.  bf16: w z goes in as the sum of three bf16 numbers, its fp32
-// value to the last bit but one: the state is an fp32 result and carries on for the whole sequence (with two of them the state of
-// 1000 tokens was off by 2.5e-6 of its norm, with one by 2.8e-3, against 4e-7 in fp32 throughout)
-template <class T> struct Weighed;
-template <> struct Weighed<float> {
+// what a chunk adds to the state: S += y^T (w z), k-step kb of it.  bf16: w z goes in as a sum of bf16 numbers, three of them (its
+// fp32 value to the last bit but one) where the state is a result of the call, in fp32, or where segments start from it; two where
+// it only meets the queries of a bf16 output.  (The final state of 1000 tokens: off by 4e-7 of its norm with three, as in fp32
+// throughout; 2.5e-6 with two, 2.8e-3 with one.)
+template <class T, int PIECES> struct Weighed;
+template <int PIECES> struct Weighed<float, PIECES> {
     f32x8 v;
     __device__ __forceinline__ Weighed(const f32x8& z, const float* w, int h) {
         const f32x4 a = *reinterpret_cast<const f32x4*>(w + 4 * h), b = *reinterpret_cast<const f32x4*>(w + 8 + 4 * h);
@@ -81,25 +83,33 @@ template <> struct Weighed<float> {
     }
     __device__ __forceinline__ f32x16 add(const f32x8& y, const f32x16& s) const { return mul(y, v, s); }
 };
-template <> struct Weighed<__bf16> {
-    bf16x8 hi, mid, lo;
+template <int PIECES> struct Weighed<__bf16, PIECES> {
+    u32x4 v[PIECES];
     __device__ __forceinline__ Weighed(const bf16x8& z, const float* w, int h) {
         const f32x4 a = *reinterpret_cast<const f32x4*>(w + 4 * h), b = *reinterpret_cast<const f32x4*>(w + 8 + 4 * h);
+        const u32x4 u = __builtin_bit_cast(u32x4, z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = (float)z[e] * (e < 4 ? a[e & 3] : b[e & 3]);
-            hi[e] = (__bf16)x;
-            const float y = x - (float)hi[e];
-            mid[e] = (__bf16)y;
-            lo[e] = (__bf16)(y - (float)mid[e]);
+        for (int e = 0; e < 4; ++e) {            // two elements at a time
+            float x = __uint_as_float(u[e] << 16) * (e < 2 ? a[2 * e] : b[2 * e - 4]);
+            float y = __uint_as_float(u[e] & 0xffff0000u) * (e < 2 ? a[2 * e + 1] : b[2 * e - 3]);
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                v[i][e] = pack2(x, y);
+                x -= __uint_as_float(v[i][e] << 16);
+                y -= __uint_as_float(v[i][e] & 0xffff0000u);
+            }
         }
     }
-    __device__ __forceinline__ f32x16 add(const bf16x8& y, const f32x16& s) const { return mul(y, hi, mul(y, mid, mul(y, lo, s))); }
+    __device__ __forceinline__ f32x16 add(const bf16x8& y, f32x16 s) const {
+#pragma unroll
+        for (int i = PIECES - 1; i >= 0; --i) s = mul(y, __builtin_bit_cast(bf16x8, v[i]), s);
+        return s;
+    }
 };
 
 // where a workgroup stands: job, head, segment
 struct Place {
-    int job, seg, h, s0, s1, send, nc;
+    int job, seg, h, s0, s1, send;
     int64_t n, nh;
     float a2;
     __device__ __forceinline__ Place(const Args& a) {
@@ -113,62 +123,117 @@ struct Place {
         s0 = seg * a.per;
         send = min(a.S, s0 + a.per);
         s1 = max(s0, min(length_of(a, n), send));
-        nc = (s1 - s0 + C - 1) / C;
     }
 };
 
-// the weights of what a chunk of m tokens adds to the state, times umul: w^{m-1-i}, from the other end w^{i+1}; zero behind m
+// the weights of what m of a chunk's 32 tokens add to the state, times umul: w^{m-1-i}, from the other end w^{i+1}; zero behind m
 __device__ __forceinline__ float add_weight(float a2, int i, int m, int rev, float umul) {
     return i < m ? umul * power(a2, rev ? i + 1 : m - 1 - i) : 0.f;
 }
 
+// the tiles of C tokens that a workgroup walks, one or two of them on their way from memory at any time
+template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
+    static constexpr int NT = 2 * DB, PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, C = TILE<T>;
+    // two sets where they take at most 48 registers each, otherwise one
+    static constexpr bool DEEP = ((OUT ? 2 : 1) * DA + DB) * C * (int)sizeof(T) <= 48 * 4 * NT;
+    static constexpr size_t LDS = ((OUT ? 2 : 1) * PA + PB) * C * sizeof(T) + C * 4;
+    struct Set {
+        al::Stage<T, DA, C, VEC, NT> x, y;
+        al::Stage<T, DB, C, VEC, NT> z;
+    };
+    const Place& at;
+    const Job& J;
+    const T *xp, *yp, *zp;
+    T *Xs, *Ys, *Zs;
+    float* wu;
+    int had = -1, nc;
+    __device__ __forceinline__ Walk(const Place& at, const Job& J, char* smem) : at(at), J(J) {
+        nc = (at.s1 - at.s0 + C - 1) / C;
+        if (OUT) xp = static_cast<const T*>(J.x) + at.n * J.sx.n + at.h * J.sx.h;
+        yp = static_cast<const T*>(J.y) + at.n * J.sy.n + at.h * J.sy.h;
+        zp = static_cast<const T*>(J.z) + at.n * J.sz.n + at.h * J.sz.h;
+        Ys = reinterpret_cast<T*>(smem);
+        Zs = Ys + C * PA;
+        Xs = Zs + C * PB;
+        wu = reinterpret_cast<float*>(Xs + (OUT ? C * PA : 0));
+    }
+    __device__ __forceinline__ void setup(Set& s, int tid) const {
+        if (OUT) s.x.setup(tid, J.sx.s, J.da);
+        s.y.setup(tid, J.sy.s, J.da);
+        s.z.setup(tid, J.sz.s, J.db);
+    }
+    __device__ __forceinline__ int tile(int t) const { return J.rev ? nc - 1 - t : t; }
+    __device__ __forceinline__ void fetch(Set& s, int t) const {                 // (past the last tile: zeros, no memory is read)
+        const int t0 = at.s0 + C * tile(t), rows = t < nc ? at.s1 - t0 : 0;
+        if (OUT) s.x.load(xp + t0 * J.sx.s, J.sx.s, rows, J.da);
+        s.y.load(yp + t0 * J.sy.s, J.sy.s, rows, J.da);
+        s.z.load(zp + t0 * J.sz.s, J.sz.s, rows, J.db);
+    }
+    // tile t into LDS; returns its token count
+    __device__ __forceinline__ int put(const Set& s, int t, int tid) {
+        const int m = min(C, at.s1 - at.s0 - C * tile(t));
+        __syncthreads();
+        if (OUT) s.x.store(Xs);
+        s.y.store(Ys);
+        s.z.store(Zs);
+        if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid & 31, min(32, max(0, m - (tid & 32))), J.rev, J.umul);
+        had = m;
+        __syncthreads();
+        return m;
+    }
+};
+// S = w^m S + sum over the m tokens of half `it` of the tile; zf: the half's z columns of this wave
+template <class T, int PA, int AT, int PIECES>
+__device__ __forceinline__ void absorb(f32x16 (&S)[AT], const T* Ys, const float* wu, const typename Ty<T>::Frag (&zf)[2], float all, int it, int lane) {
+#pragma unroll
+    for (int x = 0; x < AT; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[x][r] *= all;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const Weighed<T, PIECES> zw(zf[kb], wu + 32 * it + 16 * kb, lane >> 5);
+#pragma unroll
+        for (int x = 0; x < AT; ++x) S[x] = zw.add(col_frag<PA>(Ys, 32 * it + 16 * kb, 32 * x, lane), S[x]);
+    }
+}
+
 template <class T, int DA, int DB, bool VEC>
-__global__ __launch_bounds__(2 * DB) void lin_state_kernel(const Args a) {
-    constexpr int NT = 2 * DB, PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, AT = DA / 32;
+__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_state_kernel(const Args a) {
+    constexpr int AT = DA / 32;
+    typedef Walk<T, DA, DB, VEC, false> W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ys = reinterpret_cast<T*>(smem);
-    T* Zs = Ys + C * PA;
-    float* wu = reinterpret_cast<float*>(Zs + C * PB);
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Place at(a);
     const Job& J = a.job[at.job];
-    const T* yp = static_cast<const T*>(J.y) + at.n * J.sy.n + at.h * J.sy.h;
-    const T* zp = static_cast<const T*>(J.z) + at.n * J.sz.n + at.h * J.sz.h;
+    W walk(at, J, smem);
     f32x16 S[AT];
 #pragma unroll
     for (int t = 0; t < AT; ++t) S[t] = zero16();
-    al::Stage<T, DA, C, VEC, NT> ty;
-    al::Stage<T, DB, C, VEC, NT> tz;
-    ty.setup(tid, J.sy.s, J.da);
-    tz.setup(tid, J.sz.s, J.db);
-    auto fetch = [&](int c) {
-        const int t0 = at.s0 + C * c;
-        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da);
-        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db);
-    };
-    if (at.nc) fetch(J.rev ? at.nc - 1 : 0);
-    int had = -1;
-    for (int t = 0; t < at.nc; ++t) {
-        const int c = J.rev ? at.nc - 1 - t : t, m = min(C, at.s1 - at.s0 - C * c);
-        __syncthreads();
-        ty.store(Ys);
-        tz.store(Zs);
-        if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid, m, J.rev, J.umul);
-        had = m;
-        __syncthreads();
-        if (t + 1 < at.nc) fetch(J.rev ? c - 1 : c + 1);
-        const float all = power(at.a2, m);
+    typename W::Set s0, s1;
+    walk.setup(s0, tid);
+    walk.setup(s1, tid);
+    auto step = [&](typename W::Set& set, int t) {
+        const int m = walk.put(set, t, tid);
+        walk.fetch(set, t + (W::DEEP ? 2 : 1));
 #pragma unroll
-        for (int x = 0; x < AT; ++x)
+        for (int u = 0; u < W::C / 32; ++u) {
+            const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
+            if (mi <= 0) continue;
+            typename Ty<T>::Frag zf[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[x][r] *= all;
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            const Weighed<T> zw(col_frag<PB>(Zs, 16 * kb, 32 * w, lane), wu + 16 * kb, h);
-#pragma unroll
-            for (int x = 0; x < AT; ++x) S[x] = zw.add(col_frag<PA>(Ys, 16 * kb, 32 * x, lane), S[x]);
+            for (int kb = 0; kb < 2; ++kb) zf[kb] = col_frag<W::PB>(walk.Zs, 32 * it + 16 * kb, 32 * w, lane);
+            absorb<T, W::PA, AT, 3>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
         }
-    }
+    };
+    walk.fetch(s0, 0);
+    if (W::DEEP) {
+        walk.fetch(s1, 1);
+        for (int t = 0; t < walk.nc; t += 2) {
+            step(s0, t);
+            if (t + 1 < walk.nc) step(s1, t + 1);
+        }
+    } else
+        for (int t = 0; t < walk.nc; ++t) step(s0, t);
     float* dst = J.seg + (at.nh * a.G + at.seg) * (int64_t)(J.da * J.db);
     const int b = 32 * w + l31;
     if (b < J.db)
@@ -195,6 +260,7 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(const Args a) {
         s = J.init[nh * E + (J.init_t ? col * J.da + row : e)];
     }
     float* p = J.seg + nh * a.G * E + e;
+#pragma unroll 8
     for (int t = 0; t < a.G; ++t) {
         const int g = J.rev ? a.G - 1 - t : t;
         const int m = min(max(len - g * a.per, 0), a.per);
@@ -205,23 +271,24 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(const Args a) {
     if (J.last) J.last[nh * E + e] = s;
 }
 
-template <class T, int DA, int DB, bool VEC>
-__global__ __launch_bounds__(2 * DB) void lin_out_kernel(const Args a) {
-    constexpr int NT = 2 * DB, PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, AT = DA / 32, KA = DA / 16;
+// EXACT: one segment whose final state is wanted
+template <class T, int DA, int DB, bool VEC, bool EXACT>
+__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_out_kernel(const Args a) {
+    constexpr int NT = 2 * DB, AT = DA / 32, KA = DA / 16;
+    typedef Walk<T, DA, DB, VEC, true> W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Xs = reinterpret_cast<T*>(smem);
-    T* Ys = Xs + C * PA;
-    T* Zs = Ys + C * PA;
-    float* wu = reinterpret_cast<float*>(Zs + C * PB);
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Place at(a);
     const Job& J = a.job[at.job];
-    const T* xp = static_cast<const T*>(J.x) + at.n * J.sx.n + at.h * J.sx.h;
-    const T* yp = static_cast<const T*>(J.y) + at.n * J.sy.n + at.h * J.sy.h;
-    const T* zp = static_cast<const T*>(J.z) + at.n * J.sz.n + at.h * J.sz.h;
+    W walk(at, J, smem);
     T* op = static_cast<T*>(J.o) + at.n * J.so.n + at.h * J.so.h;
-    const int b = 32 * w + l31, rev = J.rev;
+    const int b = 32 * w + l31;
     const int64_t E = (int64_t)J.da * J.db;
+    typename W::Set set0, set1;
+    walk.setup(set0, tid);
+    walk.setup(set1, tid);
+    walk.fetch(set0, 0);
+    if (W::DEEP) walk.fetch(set1, 1);
 
     f32x16 S[AT];
     {
@@ -235,88 +302,56 @@ __global__ __launch_bounds__(2 * DB) void lin_out_kernel(const Args a) {
                 S[x][r] = src && row < J.da && b < J.db ? src[turned ? b * J.da + row : row * J.db + b] : 0.f;
             }
     }
-    // decays between the tokens of a 32 x 32 tile of scores (row j, column i = l31): on the diagonal and one tile off it
-    f32x16 near, far;
+    f32x16 near;                                 // decays between 32 tokens: row j, column i = l31
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int d = rev ? tile_row(r, h) - l31 : l31 - tile_row(r, h);
+        const int d = J.rev ? tile_row(r, h) - l31 : l31 - tile_row(r, h);
         near[r] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
-        far[r] = J.amul * power(at.a2, d + 32);
     }
-    al::Stage<T, DA, C, VEC, NT> tx, ty;
-    al::Stage<T, DB, C, VEC, NT> tz;
-    tx.setup(tid, J.sx.s, J.da);
-    ty.setup(tid, J.sy.s, J.da);
-    tz.setup(tid, J.sz.s, J.db);
-    auto fetch = [&](int c) {
-        const int t0 = at.s0 + C * c;
-        tx.load(xp + t0 * J.sx.s, J.sx.s, at.s1 - t0, J.da);
-        ty.load(yp + t0 * J.sy.s, J.sy.s, at.s1 - t0, J.da);
-        tz.load(zp + t0 * J.sz.s, J.sz.s, at.s1 - t0, J.db);
-    };
-    if (at.nc) fetch(rev ? at.nc - 1 : 0);
-    int had = -1;
-    for (int t = 0; t < at.nc; ++t) {
-        const int c = rev ? at.nc - 1 - t : t, t0 = at.s0 + C * c, m = min(C, at.s1 - t0);
-        __syncthreads();
-        tx.store(Xs);
-        ty.store(Ys);
-        tz.store(Zs);
-        if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid, m, rev, J.umul);
-        had = m;
-        __syncthreads();
-        if (t + 1 < at.nc) fetch(rev ? c - 1 : c + 1);
-        typename Ty<T>::Frag zf[4];
+    auto step = [&](typename W::Set& set, int t) {
+        const int t0 = at.s0 + W::C * walk.tile(t), m = walk.put(set, t, tid);
+        walk.fetch(set, t + (W::DEEP ? 2 : 1));
+#pragma unroll 1
+        for (int u = 0; u < W::C / 32; ++u) {
+            const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
+            if (mi <= 0) continue;
+            const T* xr = walk.Xs + (32 * it + l31) * W::PA;
+            const T* yr = walk.Ys + (32 * it + l31) * W::PA;
+            f32x16 x = zero16(), o = zero16();
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) zf[kb] = col_frag<PB>(Zs, 16 * kb, 32 * w, lane);
+            for (int k = 0; k < KA; ++k) x = mul(near_frag(yr + 16 * k + 8 * h), near_frag(xr + 16 * k + 8 * h), x);
 #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-            if (32 * it >= m) break;
-            const T* xr = Xs + (32 * it + l31) * PA;
-            f32x16 o = zero16(), os = zero16();
+            for (int y = 0; y < AT; ++y)
 #pragma unroll
-            for (int jt = 0; jt < 2; ++jt) {
-                if (rev ? jt < it : jt > it) continue;
-                f32x16 x = zero16();
-                const T* yr = Ys + (32 * jt + l31) * PA;
+                for (int k2 = 0; k2 < 2; ++k2) o = mul(tile_frag<T>(S[y], k2), spread_frag(xr + 32 * y + 16 * k2 + 4 * h), o);
+            const float wi = J.imul * power(at.a2, J.rev ? max(mi - 1 - l31, 0) : l31 + 1);
 #pragma unroll
-                for (int k = 0; k < KA; ++k) x = mul(near_frag(yr + 16 * k + 8 * h), near_frag(xr + 16 * k + 8 * h), x);
+            for (int r = 0; r < 16; ++r) { o[r] *= wi; x[r] *= near[r]; }
+            typename Ty<T>::Frag zf[2];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] *= jt == it ? near[r] : far[r];
-#pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) o = mul(zf[2 * jt + k2], tile_frag<T>(x, k2), o);
+            for (int kb = 0; kb < 2; ++kb) {
+                zf[kb] = col_frag<W::PB>(walk.Zs, 32 * it + 16 * kb, 32 * w, lane);
+                o = mul(zf[kb], tile_frag<T>(x, kb), o);
             }
-#pragma unroll
-            for (int x = 0; x < AT; ++x)
-#pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) os = mul(tile_frag<T>(S[x], k2), spread_frag(xr + 32 * x + 16 * k2 + 4 * h), os);
-            const int i = 32 * it + l31;
-            const float wi = J.imul * power(at.a2, rev ? max(m - 1 - i, 0) : i + 1);
-            if (i < m) {
-                T* row = op + (int64_t)(t0 + i) * J.so.s;
+            if (l31 < mi) {
+                T* row = op + (int64_t)(t0 + 32 * it + l31) * J.so.s;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = fmaf(wi, os[4 * q + e], o[4 * q + e]);
                     const int col = 32 * w + 8 * q + 4 * h;
-                    store4<VEC>(row + col, v, J.db - col);
+                    store4<VEC>(row + col, f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]}, J.db - col);
                 }
             }
+            absorb<T, W::PA, AT, (EXACT ? 3 : 2)>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
         }
-        const float all = power(at.a2, m);
-#pragma unroll
-        for (int x = 0; x < AT; ++x)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) S[x][r] *= all;
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            const Weighed<T> zw(zf[kb], wu + 16 * kb, h);
-#pragma unroll
-            for (int x = 0; x < AT; ++x) S[x] = zw.add(col_frag<PA>(Ys, 16 * kb, 32 * x, lane), S[x]);
+    };
+    if (W::DEEP)
+        for (int t = 0; t < walk.nc; t += 2) {
+            step(set0, t);
+            if (t + 1 < walk.nc) step(set1, t + 1);
         }
-    }
-    if (J.last && a.G == 1 && b < J.db)
+    else
+        for (int t = 0; t < walk.nc; ++t) step(set0, t);
+    if (EXACT && J.last && b < J.db)
 #pragma unroll
         for (int x = 0; x < AT; ++x)
 #pragma unroll
@@ -379,17 +414,16 @@ __global__ __launch_bounds__(256) void lin_step_kernel(const T* __restrict__ q, 
 // heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each
 static void cut(Args& a) {
     const int64_t blocks = a.jobs * a.N * a.H;
-    a.G = 1; a.per = (a.S + C - 1) / C * C;
-    if (blocks <= 0 || blocks >= 1024 || a.S <= 512) return;
-    const int64_t want = std::min<int64_t>((1024 + blocks - 1) / blocks, a.S / 256);
-    a.per = (int)((((int64_t)a.S + want - 1) / want + C - 1) / C * C);
+    a.G = 1; a.per = (a.S + UNIT - 1) / UNIT * UNIT;
+    const int64_t want = std::min<int64_t>(blocks > 0 ? 1024 / blocks : 0, a.S / 256);
+    if (want < 2) return;
+    a.per = (int)((((int64_t)a.S + want - 1) / want + UNIT - 1) / UNIT * UNIT);
     a.G = (a.S + a.per - 1) / a.per;
 }
 static int pad32(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
 template <class T, int DA, int DB, bool VEC> static int launch(const Args& a, hipStream_t s) {
-    constexpr size_t pa = DA + Ty<T>::PAD, pb = DB + Ty<T>::PAD;
-    constexpr size_t out_lds = (2 * pa + pb) * C * sizeof(T) + C * 4, state_lds = (pa + pb) * C * sizeof(T) + C * 4;
+    constexpr size_t out_lds = Walk<T, DA, DB, VEC, true>::LDS, state_lds = Walk<T, DA, DB, VEC, false>::LDS;
     const int64_t grid = a.jobs * a.N * a.H * a.G;
     NR_UNSUPPORTED(grid > 0x7fffffff, "linear_attention: %lld workgroups", (long long)grid);
     if (a.G > 1) {
@@ -402,10 +436,14 @@ template <class T, int DA, int DB, bool VEC> static int launch(const Args& a, hi
         hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)((most + 255) / 256), a.jobs), dim3(256), 0, s, a);
         if (int rc = check_launch("linear_attention scan")) return rc;
     }
-    if (out_lds > 64 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&lin_out_kernel<T, DA, DB, VEC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)out_lds);
-    hipLaunchKernelGGL((lin_out_kernel<T, DA, DB, VEC>), dim3((unsigned)grid), dim3(2 * DB), out_lds, s, a);
-    return check_launch("linear_attention");
+    bool exact = false;
+    for (int j = 0; j < a.jobs; ++j) exact = exact || (a.job[j].last && a.G == 1);
+    auto go = [&](auto kernel) {
+        if (out_lds > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)out_lds);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(2 * DB), out_lds, s, a);
+        return check_launch("linear_attention");
+    };
+    return exact ? go(&lin_out_kernel<T, DA, DB, VEC, true>) : go(&lin_out_kernel<T, DA, DB, VEC, false>);
 }
 template <class T, int DA, bool VEC> static int pick_b(const Args& a, hipStream_t s) {
     const int b = pad32(a.job[0].db);
@@ -420,7 +458,7 @@ static int run(const Args& a, bool bf16, hipStream_t s) {
     bool vec = true;
     for (int j = 0; j < a.jobs; ++j) {
         const Job& J = a.job[j];
-        vec = vec && al::aligned16(J.x, J.sx, J.da, e, C) && al::aligned16(J.y, J.sy, J.da, e, C) && al::aligned16(J.z, J.sz, J.db, e, C) && al::aligned16(J.o, J.so, J.db, e, C);
+        vec = vec && al::aligned16(J.x, J.sx, J.da, e, UNIT) && al::aligned16(J.y, J.sy, J.da, e, UNIT) && al::aligned16(J.z, J.sz, J.db, e, UNIT) && al::aligned16(J.o, J.so, J.db, e, UNIT);
     }
     return bf16 ? (vec ? pick_a<__bf16, true>(a, s) : pick_a<__bf16, false>(a, s)) : (vec ? pick_a<float, true>(a, s) : pick_a<float, false>(a, s));
 }

@@ -79,6 +79,12 @@ __device__ __forceinline__ f32x8 col_frag(const float* tile, int row0, int col0,
     return f32x8{z[0], z[PITCH], z[2 * PITCH], z[3 * PITCH], z[8 * PITCH], z[9 * PITCH], z[10 * PITCH], z[11 * PITCH]};
 }
 
+// two floats rounded to bf16 (to nearest even), the first in the low half
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
 // registers 8 kb .. 8 kb + 7 of a D tile as a fragment in "tile" order (bf16: rounded to nearest even)
 template <class T> __device__ __forceinline__ typename Ty<T>::Frag tile_frag(const f32x16& t, int kb) {
     typename Ty<T>::Frag o;
