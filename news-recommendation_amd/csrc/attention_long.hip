@@ -99,11 +99,11 @@ int attn_long_bwd(const AttnProblem& p, const AttnGrad& g, void* ws, size_t ws_b
     al::Args a = al::make_args(p);
     a.out = const_cast<void*>(g.out); a.so = g.so; a.dout = g.dout; a.sdo = g.sdo;
     a.row_max = const_cast<float*>(g.row_max); a.row_sum = const_cast<float*>(g.row_sum);
-    a.delta = g.delta; a.sd = g.sd;
+    a.delta = g.delta; a.sd = g.sd; a.keep_delta = static_cast<const void*>(g.delta) != g.dq;
     a.dq = g.dq; a.dk = g.dk; a.dv = g.dv; a.sdq = g.sdq; a.sdk = g.sdk; a.sdv = g.sdv;
     a.part = static_cast<float*>(ws);
     const size_t e = p.bf16 ? 2 : 4;
-    const bool vec = al::all_aligned(p) && al::aligned16(g.dout, g.sdo, p.dh, e, 128) && al::aligned16(g.dq, g.sdq, p.dh, e, 128);
+    const bool vec = al::all_aligned(p) && al::aligned16(g.dout, g.sdo, p.dh, e, 128) && al::aligned16(g.out, g.so, p.dh, e, 128) && al::aligned16(g.dq, g.sdq, p.dh, e, 128);
     const bool room = !f.ws || (ws && ws_bytes >= f.ws), drop = p.dc.p > 0.f;      // without room for the partial sums nothing is split
     return p.bf16 ? al::run_bwd<__bf16>(a, f, vec, drop, room, s) : al::run_bwd<float>(a, f, vec, drop, room, s);
 }

@@ -9,7 +9,8 @@
 //     dV += P^T dO and dK += dS^T Q.
 //   dQ: a wave owns 32 rows and walks the keys, as in the forward; dS^T is the B operand of dQ^T += K^T dS^T.
 // The two recompute S and dP: 14 products of 2 * pairs * dh operations where one pass with atomics needs 10.
-// delta comes from a small kernel before both.
+// delta: the dQ pass forms it from the rows it holds anyway and, running first, leaves it for the other; where it has no place of
+// its own but lies in dQ's rows (attention_long.h), a small kernel writes it there, the dK / dV pass reads it and dQ goes last.
 #pragma once
 #include "attention_long_dev.h"
 
@@ -45,7 +46,7 @@ template <class T, int DHP> struct DkvCfg {
     static constexpr int QSUB = sizeof(T) == 2 ? 2 : 1, QT = 32 * QSUB, PITCH = DHP + Ty<T>::PAD;
     static constexpr size_t TILES = (size_t)2 * 2 * QT * PITCH * sizeof(T);
     static constexpr size_t BYTES = TILES + (size_t)2 * 3 * QT * 4;              // + two stages of the rows' statistics
-    static constexpr int WAVES = DHP <= 64 ? 2 : 1;
+    static constexpr int WAVES = DHP <= 64 ? (sizeof(T) == 2 ? 3 : 2) : 1;
 };
 
 template <class T, int DHP, bool VEC, bool DROP>
@@ -88,15 +89,16 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
     // the tiles of this block: per query head those from the first position that reaches the block's keys on, cut evenly over the splits
     const int tq = (a.Sq + QT - 1) / QT, t0 = a.causal ? min(tq, max(0, kb * 128 - off) / QT) : 0, per = tq - t0;
     const int64_t all = (int64_t)a.rep * per;
-    int u = (int)(all * sp / a.splits);
-    const int uend = __syncthreads_or(there) ? (int)(all * (sp + 1) / a.splits) : u;      // no key of this block is there: nothing to add
+    const int ubeg = (int)(all * sp / a.splits);
+    const int left = __syncthreads_or(there) ? (int)(all * (sp + 1) / a.splits) - ubeg : 0;      // no key of this block is there: nothing to add
+    int hh = per ? ubeg / per : 0, i0 = (t0 + ubeg - hh * per) * QT;             // query head (of the key head's) and first position of the tile
 
     Stage<T, DHP, QT, VEC> sq, sg;
     sq.setup(tid, a.sq.s, a.dh);
     sg.setup(tid, a.sdo.s, a.dh);
     float st[3];
-    auto fetch = [&](int u) {
-        const int hh = per ? u / per : 0, i0 = (t0 + u - hh * per) * QT, head = g * a.rep + hh, rows = u < uend ? a.Sq - i0 : 0;
+    auto fetch = [&](int hh, int i0, bool any) {
+        const int head = g * a.rep + hh, rows = any ? a.Sq - i0 : 0;
         sq.load(static_cast<const T*>(a.q) + n * a.sq.n + i0 * a.sq.s + head * a.sq.h, a.sq.s, rows, a.dh);
         sg.load(static_cast<const T*>(a.dout) + n * a.sdo.n + i0 * a.sdo.s + head * a.sdo.h, a.sdo.s, rows, a.dh);
         if (tid < QT) {
@@ -120,16 +122,18 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         }
     };
     int buf = 0;
-    if (u < uend) { fetch(u); put(0); }
+    if (left > 0) { fetch(hh, i0, true); put(0); }
     __syncthreads();
-    for (; u < uend; ++u) {
-        const int hh = u / per, i0 = (t0 + u - hh * per) * QT;
-        fetch(u + 1);
+    for (int u = 0; u < left; ++u) {
+        int hh1 = hh, i1 = i0 + QT;
+        if (i1 >= a.Sq) { ++hh1; i1 = t0 * QT; }
+        fetch(hh1, i1, u + 1 < left);
         const T* Qt = Qs + buf * QT * PITCH;
         const T* Gt = Gs + buf * QT * PITCH;
         const float* S0 = St + buf * 3 * QT;
         if (alive && !(a.causal && i0 + QT - 1 + off < key0)) {
-#pragma unroll
+            // not unrolled: with both halves' reads in flight the kernel ran out of registers (4001 x 128 causal: 261 us against 225)
+#pragma unroll 1
             for (int s = 0; s < QSUB; ++s) {
                 f32x16 x = zero16(), dp = zero16();
                 const T* qr = Qt + (32 * s + l31) * PITCH + 8 * h;
@@ -183,6 +187,7 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         put(buf ^ 1);
         __syncthreads();
         buf ^= 1;
+        hh = hh1; i0 = i1;
     }
     const int64_t total = a.N * a.G * a.Sk;
     T* dkp = static_cast<T*>(a.dk) + n * a.sdk.n + g * a.sdk.h;
@@ -257,7 +262,17 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
         rl = a.row_sum[x];
         if (NAT) rl = 1.f / rl;
         else m = m * LOG2E + __builtin_amdgcn_logf(rl);
-        de = a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h];
+    }
+    {   // delta of the row, from its output and gradient; kept for the dK / dV pass if that one follows
+        const T* op = static_cast<const T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const typename Ty<T>::Frag of = load_frag<VEC>(op + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) de = fmaf((float)of[e], (float)gf[ks][e], de);
+        }
+        de += __shfl_xor(de, 32, 64);
+        if (a.keep_delta && live && h == 0 && wk == 0 && sp == 0) a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h] = de;
     }
     int begin = sp * a.per_split, stop = min(a.Sk, begin + a.per_split);
     if (a.causal) {
@@ -280,8 +295,14 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
     KeyBits kb;
     kb.words = reinterpret_cast<uint64_t*>(smem + C::BITS);
     kb.masked = mask != nullptr;
-    for (; begin < stop; begin += SPAN) {
-        int end = stop;
+    int end = stop;
+    auto fetch = [&](int j) {
+        sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
+        sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
+    };
+    for (; begin < stop; begin += SPAN) {        // (one turn without a mask)
+        end = stop;
+        fetch(begin);                            // on its way while the key bits are read
         kb.from = begin;
         kb.end = stop;
         if (mask) {
@@ -289,10 +310,6 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
             const int there = kb.fill(mask, lane, w);
             if (cut) kb.end = end = there;
         }
-        auto fetch = [&](int j) {
-            sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
-            sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
-        };
         auto put = [&](int buf, int j) {
             uint64_t bits[WORDS];
             bool all = true;
@@ -311,7 +328,7 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
             }
         };
         const int tiles = (end - begin + KT - 1) / KT;
-        if (tiles > 0) { fetch(begin); put(0, begin); }
+        if (tiles > 0) put(0, begin);
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
@@ -472,21 +489,35 @@ template <class T> static int run_sum(const Args& a, int which, hipStream_t s) {
 }
 template <class T, bool DROP>
 static int passes(Args a, const BwdPlan& f, bool vec, bool room, hipStream_t s) {
-    a.nblk = f.nblk_k; a.splits = room ? f.kv.splits : 1;
-    unsigned grid = (unsigned)(a.N * a.G * (int64_t)a.nblk * a.splits);
-    if (int rc = vec ? pick_dkv<T, true, DROP>(a, grid, s) : pick_dkv<T, false, DROP>(a, grid, s)) return rc;
-    if (int rc = run_sum<T>(a, 1, s)) return rc;
-    a.nblk = f.nblk_q; a.head_blocks = f.head_blocks; a.splits = room ? f.q.splits : 1; a.per_split = room ? f.q.per : a.Sk;
-    grid = (unsigned)(a.N * a.G * (int64_t)a.nblk * a.splits);
-    int rc = f.wk == 4 ? (vec ? pick_dq<T, true, 4, DROP>(a, grid, s) : pick_dq<T, false, 4, DROP>(a, grid, s))
-                       : (vec ? pick_dq<T, true, 1, DROP>(a, grid, s) : pick_dq<T, false, 1, DROP>(a, grid, s));
-    return rc != NR_OK ? rc : run_sum<T>(a, 0, s);
+    auto keys = [&]() {
+        Args b = a;
+        b.nblk = f.nblk_k; b.splits = room ? f.kv.splits : 1;
+        const unsigned grid = (unsigned)(b.N * b.G * (int64_t)b.nblk * b.splits);
+        if (int rc = vec ? pick_dkv<T, true, DROP>(b, grid, s) : pick_dkv<T, false, DROP>(b, grid, s)) return rc;
+        return run_sum<T>(b, 1, s);
+    };
+    auto rows = [&]() {
+        Args b = a;
+        b.nblk = f.nblk_q; b.head_blocks = f.head_blocks; b.splits = room ? f.q.splits : 1; b.per_split = room ? f.q.per : a.Sk;
+        const unsigned grid = (unsigned)(b.N * b.G * (int64_t)b.nblk * b.splits);
+        const int rc = f.wk == 4 ? (vec ? pick_dq<T, true, 4, DROP>(b, grid, s) : pick_dq<T, false, 4, DROP>(b, grid, s))
+                                 : (vec ? pick_dq<T, true, 1, DROP>(b, grid, s) : pick_dq<T, false, 1, DROP>(b, grid, s));
+        return rc != NR_OK ? rc : run_sum<T>(b, 0, s);
+    };
+    if (a.keep_delta) {
+        const int rc = rows();
+        return rc != NR_OK ? rc : keys();
+    }
+    const int rc = keys();
+    return rc != NR_OK ? rc : rows();
 }
 template <class T>
 int run_bwd(Args a, const BwdPlan& f, bool vec, bool drop, bool room, hipStream_t s) {
-    const int64_t rows = a.N * a.Sq * a.H;
-    hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows * 16 + 255) / 256)), dim3(256), 0, s, a);
-    if (int rc = check_launch("attention_bwd delta")) return rc;
+    if (!a.keep_delta) {
+        const int64_t rows = a.N * a.Sq * a.H;
+        hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows * 16 + 255) / 256)), dim3(256), 0, s, a);
+        if (int rc = check_launch("attention_bwd delta")) return rc;
+    }
     return drop ? passes<T, true>(a, f, vec, room, s) : passes<T, false>(a, f, vec, room, s);
 }
 

@@ -26,6 +26,7 @@ struct Args {
     // backward
     const void* dout; AttnStrides sdo;
     float* delta; AttnStrides sd;
+    int keep_delta;                             // the dQ pass runs first and writes delta
     void *dq, *dk, *dv; AttnStrides sdq, sdk, sdv;
     // split of the long axis
     float* part; float* part_ml;

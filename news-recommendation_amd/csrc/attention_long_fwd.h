@@ -92,8 +92,14 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
     KeyBits kb;
     kb.words = reinterpret_cast<uint64_t*>(smem + C::BITS);
     kb.masked = mask != nullptr;
+    int end = stop;
+    auto fetch = [&](int j) {
+        sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
+        sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
+    };
     for (; begin < stop; begin += SPAN) {        // (one turn without a mask)
-        int end = stop;
+        end = stop;
+        fetch(begin);                            // on its way while the key bits are read
         kb.from = begin;
         kb.end = stop;
         if (mask) {
@@ -101,10 +107,6 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
             const int there = kb.fill(mask, lane, w);
             if (cut) kb.end = end = there;
         }
-        auto fetch = [&](int j) {
-            sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
-            sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
-        };
         auto put = [&](int buf, int j) {
             // an absent key's row reads as zero: whatever its memory holds (a NaN as well) must not reach 0 * v
             uint64_t bits[WORDS];
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
             }
         };
         const int tiles = (end - begin + KT - 1) / KT;
-        if (tiles > 0) { fetch(begin); put(0, begin); }
+        if (tiles > 0) put(0, begin);
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;

@@ -6,6 +6,7 @@ the product's ops raises.  The library is built in-tree by
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnewsrec_hip.so")
@@ -42,15 +43,10 @@ class TfmSavedBf16(C.Structure):
     _fields_ = [(n, c_fp) for n in ("x_h", "qkv_h", "ctx_h", "y1_h", "z_h", "a_h", "s1", "y1", "s2", "stats", "row_max", "row_sum", "w_h", "wT_h")]
 
 
-class Attention(C.Structure):
-    _fields_ = ([(n, c_fp) for n in ("q", "k", "v", "key_mask")] + [(n, c_i64) for n in ("N", "Sq", "Sk", "H", "G", "dh")] +
-                [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")] +
-                [("dtype", C.c_int32), ("causal", C.c_int32), ("scale", c_f), ("p_drop", c_f), ("seed", c_u64), ("site", c_u32)])
-
-
-class LinearAttention(C.Structure):
-    _fields_ = ([(n, c_fp) for n in ("q", "k", "v", "log_decay", "lens", "state")] + [(n, c_i64) for n in ("N", "S", "H", "dk", "dv")] +
-                [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("dtype", C.c_int32), ("scale", c_f)])
+# nr_attention and nr_linear_attention (include/newsrec_hip.h) as packed bytes: a call passes one by address, and a Struct packs one in
+# a fraction of the time that a ctypes.Structure with its arrays takes to build (a single-query call is bound by its host side)
+ATTENTION = struct.Struct("=4Q6q9q2i2fQI4x")
+LINEAR_ATTENTION = struct.Struct("=6Q5q9qif")
 
 
 _SIGS = {
@@ -88,14 +84,14 @@ _SIGS = {
     "nr_mhsa_bwd_bf16": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_i64, c_f, c_u64, c_u32, c_int, c_fp, c_fp]),
     "nr_mhsa_bwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_fp, c_fp, c_i64, c_i64, c_i64, c_i64, c_f, c_u64, c_u32, c_int,
                                 c_fp, c_fp]),
-    "nr_attention_fwd_ws_bytes": (c_sz, [C.POINTER(Attention)]),
-    "nr_attention_fwd": (c_int, [C.POINTER(Attention), c_fp, c_fp, c_fp, c_fp, c_sz, c_fp]),
-    "nr_attention_bwd_ws_bytes": (c_sz, [C.POINTER(Attention)]),
-    "nr_attention_bwd": (c_int, [C.POINTER(Attention)] + [c_fp] * 9 + [c_sz, c_fp]),
-    "nr_linear_attention_fwd_ws_bytes": (c_sz, [C.POINTER(LinearAttention)]),
-    "nr_linear_attention_fwd": (c_int, [C.POINTER(LinearAttention), c_fp, c_fp, c_fp, c_sz, c_fp]),
-    "nr_linear_attention_bwd_ws_bytes": (c_sz, [C.POINTER(LinearAttention)]),
-    "nr_linear_attention_bwd": (c_int, [C.POINTER(LinearAttention)] + [c_fp] * 7 + [c_sz, c_fp]),
+    "nr_attention_fwd_ws_bytes": (c_sz, [C.c_char_p]),
+    "nr_attention_fwd": (c_int, [C.c_char_p, c_fp, c_fp, c_fp, c_fp, c_sz, c_fp]),
+    "nr_attention_bwd_ws_bytes": (c_sz, [C.c_char_p]),
+    "nr_attention_bwd": (c_int, [C.c_char_p] + [c_fp] * 9 + [c_sz, c_fp]),
+    "nr_linear_attention_fwd_ws_bytes": (c_sz, [C.c_char_p]),
+    "nr_linear_attention_fwd": (c_int, [C.c_char_p, c_fp, c_fp, c_fp, c_sz, c_fp]),
+    "nr_linear_attention_bwd_ws_bytes": (c_sz, [C.c_char_p]),
+    "nr_linear_attention_bwd": (c_int, [C.c_char_p] + [c_fp] * 7 + [c_sz, c_fp]),
     "nr_linear_attention_step": (c_int, [c_fp] * 5 + [c_i64] * 4 + [c_int, c_f, c_fp, c_fp, c_fp]),
     "nr_query_pool_fwd_f32": (c_int, [c_fp, c_fp, c_fp, c_fp, c_i64, c_fp, c_fp, c_i64, c_i64, c_i64, c_fp, c_fp, c_fp]),
     "nr_query_pool_bwd_ws_bytes": (c_sz, [c_i64, c_i64]),

@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import Attention, LinearAttention, NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
+from ._lib import ATTENTION, LINEAR_ATTENTION, NewsrecError, TfmWeights, TfmGrads, TfmSaved, TfmSavedBf16, check
 
 PAD_ID = 0          # BERT word_embeddings.padding_idx (manager.special_token_ids["[PAD]"])
 LN_EPS = 1e-12      # models/modules/attention.py:106,151 of the reference
@@ -479,7 +479,7 @@ def _seq(t, name, dims, like=None):
         raise NewsrecError(f"{name}: expected {dims} axes, got {tuple(t.shape)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise NewsrecError(f"{name}: {t.dtype} on {t.device}, but the other operands are {like.dtype} on {like.device}")
-    return t if t.numel() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 or t.numel() == 0 else t.contiguous()
 
 
 def _same_device(t, name, device):
@@ -488,63 +488,72 @@ def _same_device(t, name, device):
     return t
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on_device(t):
     """the kernels run on the current device's current stream: make `t`'s device the current one"""
     if _cur_device is not None and _cur_device() == t.device.index:
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(t.device)
 
 
 def _attention_problem(q, k, v, mask, causal, scale, p, seed, site):
-    (N, Sq, H, dh), (Sk, G) = q.shape, k.shape[1:3]
-    three = C.c_int64 * 3
-    return Attention(_p(q), _p(k), _p(v), _p(mask), N, Sq, Sk, H, G, dh, three(*q.stride()[:3]), three(*k.stride()[:3]), three(*v.stride()[:3]),
-                     _SEQ_TYPES[q.dtype], int(causal), scale, p, seed, site)
+    N, Sq, H, dh = q.shape
+    _, Sk, G, _ = k.shape
+    return ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if mask is None else mask.data_ptr(), N, Sq, Sk, H, G, dh,
+                          *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _SEQ_TYPES[q.dtype], causal, scale, p, seed, site)
+
+
+def _attention_fwd(q, k, v, mask, cfg, train):
+    """(out, row_max, row_sum); the statistics are None unless a backward is to follow"""
+    N, Sq, H, dh = q.shape
+    out = torch.empty((N, Sq, H, dh), dtype=q.dtype, device=q.device)
+    if out.numel() == 0 or k.shape[1] == 0:
+        return out.zero_(), None, None
+    rmax = rsum = ws = None
+    if train:
+        rmax = torch.empty((N, H, Sq), dtype=torch.float32, device=q.device)
+        rsum = torch.empty((N, H, Sq), dtype=torch.float32, device=q.device)
+    L = lib()
+    with _on_device(q):
+        P = _attention_problem(q, k, v, mask, *cfg)
+        nbytes = L.nr_attention_fwd_ws_bytes(P)
+        if nbytes:
+            ws = _ws(nbytes, q.device)
+        check(L.nr_attention_fwd(P, out.data_ptr(), _p(rmax), _p(rsum), _p(ws), nbytes, _stream()), "nr_attention_fwd")
+    return out, rmax, rsum
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, causal, scale, p, seed, site, grad_mode):
-        N, Sq, H, dh = q.shape
-        out = torch.empty(N, Sq, H, dh, dtype=q.dtype, device=q.device)
+    def forward(ctx, q, k, v, mask, cfg):
         ctx.set_materialize_grads(False)
-        ctx.cfg = (causal, scale, p, seed, site)
-        if out.numel() == 0 or k.shape[1] == 0:
-            ctx.save_for_backward(q, k, v, mask, None, None, None)
-            return out.zero_()
-        train = grad_mode and any(ctx.needs_input_grad[:3])      # (see _TFMLayer.forward)
-        rmax = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device) if train else None
-        rsum = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device) if train else None
-        L = lib()
-        with _on_device(q):
-            P = _attention_problem(q, k, v, mask, *ctx.cfg)
-            nbytes = L.nr_attention_fwd_ws_bytes(C.byref(P))
-            ws = _ws(nbytes, q.device) if nbytes else None
-            check(L.nr_attention_fwd(C.byref(P), _p(out), _p(rmax), _p(rsum), _p(ws), nbytes, _stream()), "nr_attention_fwd")
-        if train:
-            ctx.save_for_backward(q, k, v, mask, out, rmax, rsum)
+        ctx.cfg = cfg
+        out, rmax, rsum = _attention_fwd(q, k, v, mask, cfg, True)
+        ctx.save_for_backward(q, k, v, mask, out if rmax is not None else None, rmax, rsum)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         if g is None:
-            return (None,) * 10
+            return (None,) * 5
         q, k, v, mask, out, rmax, rsum = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        if out is None:
-            return (dq.zero_(), dk.zero_(), dv.zero_()) + (None,) * 7
+        if out is None:                          # an empty axis: nothing was computed, every gradient is zero
+            return dq.zero_(), dk.zero_(), dv.zero_(), None, None
         g = g.contiguous()
         N, Sq, H, _ = q.shape
         delta = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device)
         L = lib()
         with _on_device(q):
             P = _attention_problem(q, k, v, mask, *ctx.cfg)
-            nbytes = L.nr_attention_bwd_ws_bytes(C.byref(P))
+            nbytes = L.nr_attention_bwd_ws_bytes(P)
             ws = _ws(nbytes, q.device) if nbytes else None
-            check(L.nr_attention_bwd(C.byref(P), _p(out), _p(g), _p(rmax), _p(rsum), _p(delta), _p(dq), _p(dk), _p(dv), _p(ws), nbytes,
+            check(L.nr_attention_bwd(P, _p(out), _p(g), _p(rmax), _p(rsum), _p(delta), _p(dq), _p(dk), _p(dv), _p(ws), nbytes,
                                      _stream()), "nr_attention_bwd")
-        return (dq, dk, dv) + (None,) * 7
+        return dq, dk, dv, None, None
 
 
 def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed=0, site=0):
@@ -572,7 +581,10 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
         raise NewsrecError(f"attention: scale {scale} is not a positive number")
     if not 0.0 <= p_drop < 1.0:
         raise NewsrecError(f"attention: p_drop {p_drop} not in [0, 1)")
-    return _Attention.apply(q, k, v, key_mask, bool(causal), scale, float(p_drop), int(seed), int(site), torch.is_grad_enabled())
+    cfg = (1 if causal else 0, scale, float(p_drop), int(seed), int(site))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, key_mask, cfg)
+    return _attention_fwd(q, k, v, key_mask, cfg, False)[0]
 
 
 # ----------------------------------------------------------------------------- conv1d(k=3, pad=1) + relu
@@ -852,24 +864,29 @@ def gru_final_state(x, mask, w_ih, w_hh, b_ih, b_hh):
 
 # ----------------------------------------------------------------------------- linear attention with a decay per head
 def _linear_problem(q, k, v, log_decay, lens, state, scale):
+    N, S, H, dk = q.shape
+    return LINEAR_ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), 0 if lens is None else lens.data_ptr(),
+                                 0 if state is None else state.data_ptr(), N, S, H, dk, v.shape[3], *q.stride()[:3], *k.stride()[:3],
+                                 *v.stride()[:3], _SEQ_TYPES[q.dtype], scale)
+
+
+def _linear_fwd(q, k, v, log_decay, lens, state, scale):
     (N, S, H, dk), dv = q.shape, v.shape[3]
-    three = C.c_int64 * 3
-    return LinearAttention(_p(q), _p(k), _p(v), _p(log_decay), _p(lens), _p(state), N, S, H, dk, dv, three(*q.stride()[:3]),
-                           three(*k.stride()[:3]), three(*v.stride()[:3]), _SEQ_TYPES[q.dtype], scale)
+    out = torch.empty((N, S, H, dv), dtype=q.dtype, device=q.device)
+    last = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device)
+    L = lib()
+    with _on_device(q):
+        P = _linear_problem(q, k, v, log_decay, lens, state, scale)
+        nbytes = L.nr_linear_attention_fwd_ws_bytes(P)
+        ws = _ws(nbytes, q.device) if nbytes else None
+        check(L.nr_linear_attention_fwd(P, _p(out), _p(last), _p(ws), nbytes, _stream()), "nr_linear_attention_fwd")
+    return out, last
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, lens, state, scale):
-        (N, S, H, dk), dv = q.shape, v.shape[3]
-        out = torch.empty(N, S, H, dv, dtype=q.dtype, device=q.device)
-        last = torch.empty(N, H, dk, dv, dtype=torch.float32, device=q.device)
-        L = lib()
-        with _on_device(q):
-            P = _linear_problem(q, k, v, log_decay, lens, state, scale)
-            nbytes = L.nr_linear_attention_fwd_ws_bytes(C.byref(P))
-            ws = _ws(nbytes, q.device) if nbytes else None
-            check(L.nr_linear_attention_fwd(C.byref(P), _p(out), _p(last), _p(ws), nbytes, _stream()), "nr_linear_attention_fwd")
+        out, last = _linear_fwd(q, k, v, log_decay, lens, state, scale)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, v, log_decay, lens, state)
         ctx.scale = scale
@@ -889,9 +906,9 @@ class _LinearAttention(torch.autograd.Function):
         L = lib()
         with _on_device(q):
             P = _linear_problem(q, k, v, log_decay, lens, state, ctx.scale)
-            nbytes = L.nr_linear_attention_bwd_ws_bytes(C.byref(P))
+            nbytes = L.nr_linear_attention_bwd_ws_bytes(P)
             ws = _ws(nbytes, q.device) if nbytes else None
-            check(L.nr_linear_attention_bwd(C.byref(P), _p(g), _p(glast), _p(dq), _p(dk_), _p(dv_), _p(dstate), _p(ws), nbytes, _stream()),
+            check(L.nr_linear_attention_bwd(P, _p(g), _p(glast), _p(dq), _p(dk_), _p(dv_), _p(dstate), _p(ws), nbytes, _stream()),
                   "nr_linear_attention_bwd")
         return dq, dk_, dv_, None, None, dstate, None
 
@@ -930,10 +947,11 @@ def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
         lens = _same_device(_i64(lens, "lens"), "lens", q.device)
         if tuple(lens.shape) != (q.shape[0],):
             raise NewsrecError(f"linear_attention: lens {tuple(lens.shape)} for {q.shape[0]} sequences")
-    return _LinearAttention.apply(q, k, v, log_decay, lens, state, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+        return _LinearAttention.apply(q, k, v, log_decay, lens, state, scale)
+    return _linear_fwd(q, k, v, log_decay, lens, state, scale)
 
 
-@torch.no_grad()
 def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None):
     """one token of linear_attention for every sequence: q / k [N,H,dk], v [N,H,dv], state [N,H,dk,dv] fp32 -> o [N,H,dv].  The new
     state goes to out_state (dense, may be state itself), by default over state.  Inference only (no autograd)."""
@@ -950,7 +968,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     N, H, dk = q.shape
     dv = v.shape[2]
-    out = torch.empty(N, H, dv, dtype=q.dtype, device=q.device)
+    out = torch.empty((N, H, dv), dtype=q.dtype, device=q.device)
     with _on_device(q):
         check(lib().nr_linear_attention_step(_p(q), _p(k), _p(v), _p(log_decay), _p(state), N, H, dk, dv, _SEQ_TYPES[q.dtype], scale, _p(out),
                                              _p(out_state), _stream()), "nr_linear_attention_step")
