@@ -43,8 +43,10 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const Args a) {
 // ---------------------------------------------------------------- dK, dV
 // a tile holds QT positions of one query head; the tiles of all query heads of the key head follow one another
 template <class T, int DHP> struct DkvCfg {
-    static constexpr int QSUB = sizeof(T) == 2 ? 2 : 1, QT = 32 * QSUB, PITCH = DHP + Ty<T>::PAD;
-    static constexpr size_t TILES = (size_t)2 * 2 * QT * PITCH * sizeof(T);
+    static constexpr int QSUB = sizeof(T) == 2 ? 2 : 1, QT = 32 * QSUB;
+    typedef typename MulType<T, 1>::M M;
+    typedef Lds<M, QT, DHP> L;
+    static constexpr size_t TILES = 2 * 2 * L::BYTES;
     static constexpr size_t BYTES = TILES + (size_t)2 * 3 * QT * 4;              // + two stages of the rows' statistics
     static constexpr int WAVES = DHP <= 64 ? (sizeof(T) == 2 ? 3 : 2) : 1;
 };
@@ -52,11 +54,13 @@ template <class T, int DHP> struct DkvCfg {
 template <class T, int DHP, bool VEC, bool DROP>
 __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(const Args a) {
     typedef DkvCfg<T, DHP> C;
-    constexpr int QSUB = C::QSUB, QT = C::QT, PITCH = C::PITCH, KS = DHP / 16, DT = DHP / 32;
+    constexpr int QSUB = C::QSUB, QT = C::QT, KS = DHP / 16, DT = DHP / 32;
     constexpr bool NAT = sizeof(T) == 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Qs = reinterpret_cast<T*>(smem);
-    T* Gs = Qs + 2 * QT * PITCH;
+    typedef typename C::M M;
+    typedef typename C::L L;
+    char* Qs = smem;
+    char* Gs = smem + 2 * L::BYTES;
     float* St = reinterpret_cast<float*>(smem + C::TILES);                       // [2][3][QT]: fp32 m, 1 / l, delta; bf16 log2(l e^m), -, delta
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -69,14 +73,14 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
     const bool masked = there && a.mask && a.mask[n * a.Sk + key] == 0;
     const float sink = masked ? a.fill : 0.f;                                    // additive mode
     if (!a.additive && masked) there = false;
-    typename Ty<T>::Frag kf[KS], vf[KS];
+    typename Ty<M>::Frag kf[KS], vf[KS];
     {   // an absent key's rows read as zero.  (What its scores then give stays in its own rows of dK and dV, which are written as zero.)
         const T* kp = static_cast<const T*>(a.k) + n * a.sk.n + (int64_t)key * a.sk.s + g * a.sk.h;
         const T* vp = static_cast<const T*>(a.v) + n * a.sv.n + (int64_t)key * a.sv.s + g * a.sv.h;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            kf[ks] = load_frag<VEC>(kp + 16 * ks + 8 * h, there ? a.dh - 16 * ks - 8 * h : 0);
-            vf[ks] = load_frag<VEC>(vp + 16 * ks + 8 * h, there ? a.dh - 16 * ks - 8 * h : 0);
+            kf[ks] = As<M>::frag(load_frag<VEC>(kp + 16 * ks + 8 * h, there ? a.dh - 16 * ks - 8 * h : 0));
+            vf[ks] = As<M>::frag(load_frag<VEC>(vp + 16 * ks + 8 * h, there ? a.dh - 16 * ks - 8 * h : 0));
         }
     }
     f32x16 dk[DT], dv[DT];
@@ -112,8 +116,8 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         }
     };
     auto put = [&](int buf) {
-        sq.store(Qs + buf * QT * PITCH);
-        sg.store(Gs + buf * QT * PITCH);
+        sq.template store<L>(Qs + buf * L::BYTES);
+        sg.template store<L>(Gs + buf * L::BYTES);
         if (tid < QT) {
             float* s = St + buf * 3 * QT + tid;
             if (NAT) { s[0] = st[0]; s[QT] = 1.f / st[1]; }
@@ -128,20 +132,18 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         int hh1 = hh, i1 = i0 + QT;
         if (i1 >= a.Sq) { ++hh1; i1 = t0 * QT; }
         fetch(hh1, i1, u + 1 < left);
-        const T* Qt = Qs + buf * QT * PITCH;
-        const T* Gt = Gs + buf * QT * PITCH;
+        const char* Qt = Qs + buf * L::BYTES;
+        const char* Gt = Gs + buf * L::BYTES;
         const float* S0 = St + buf * 3 * QT;
         if (alive && !(a.causal && i0 + QT - 1 + off < key0)) {
             // not unrolled: with both halves' reads in flight the kernel ran out of registers (4001 x 128 causal: 261 us against 225)
 #pragma unroll 1
             for (int s = 0; s < QSUB; ++s) {
                 f32x16 x = zero16(), dp = zero16();
-                const T* qr = Qt + (32 * s + l31) * PITCH + 8 * h;
-                const T* gr = Gt + (32 * s + l31) * PITCH + 8 * h;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    x = mul(near_frag(qr + 16 * ks), kf[ks], x);
-                    dp = mul(near_frag(gr + 16 * ks), vf[ks], dp);
+                    x = mul(L::near(Qt, 32 * s + l31, 16 * ks + 8 * h), kf[ks], x);
+                    dp = mul(L::near(Gt, 32 * s + l31, 16 * ks + 8 * h), vf[ks], dp);
                 }
                 if (a.causal && i0 + 32 * s + off < key0 + 31) {                 // the diagonal: row i sees the key if i + off >= key
                     const int first = key - off - (i0 + 32 * s) - 4 * h;
@@ -175,11 +177,11 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
                 }
 #pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) {
-                    const typename Ty<T>::Frag pf = tile_frag<T>(x, k2), sf = tile_frag<T>(dp, k2);
+                    const typename Ty<M>::Frag pf = tile_frag<M>(x, k2), sf = tile_frag<M>(dp, k2);
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        dv[d] = mul(pf, col_frag<PITCH>(Gt, 32 * s + 16 * k2, 32 * d, lane), dv[d]);
-                        dk[d] = mul(sf, col_frag<PITCH>(Qt, 32 * s + 16 * k2, 32 * d, lane), dk[d]);
+                        dv[d] = mul(pf, L::col(Gt, 32 * s + 16 * k2, 32 * d, lane), dv[d]);
+                        dk[d] = mul(sf, L::col(Qt, 32 * s + 16 * k2, 32 * d, lane), dk[d]);
                     }
                 }
             }
@@ -216,9 +218,11 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
 
 // ---------------------------------------------------------------- dQ
 template <class T, int DHP, int WK> struct DqCfg {
-    static constexpr int KSUB = (sizeof(T) == 2 && WK == 1) ? 2 : 1, KT = 32 * KSUB * WK, PITCH = DHP + Ty<T>::PAD;
+    static constexpr int KSUB = (sizeof(T) == 2 && WK == 1) ? 2 : 1, KT = 32 * KSUB * WK;
+    typedef typename MulType<T, WK>::M M;
+    typedef Lds<M, KT, DHP> L;
     static constexpr int NBUF = (sizeof(T) == 4 && DHP == 128 && WK == 4) ? 1 : 2;
-    static constexpr size_t TILES = (size_t)NBUF * 2 * KT * PITCH * sizeof(T);
+    static constexpr size_t TILES = NBUF * 2 * L::BYTES;
     static constexpr size_t JOIN = WK > 1 ? (size_t)WK * DHP * 32 * 4 : 0;
     static constexpr size_t BITS = TILES > JOIN ? TILES : JOIN, BYTES = BITS + SPAN / 8;
     static constexpr int WAVES = BYTES <= 80 * 1024 && DHP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1;
@@ -227,11 +231,13 @@ template <class T, int DHP, int WK> struct DqCfg {
 template <class T, int DHP, bool VEC, int WK, bool DROP>
 __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kernel(const Args a) {
     typedef DqCfg<T, DHP, WK> C;
-    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, PITCH = C::PITCH, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
+    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
     constexpr bool NAT = sizeof(T) == 4;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + C::NBUF * KT * PITCH;
+    typedef typename C::M M;
+    typedef typename C::L L;
+    char* Ks = smem;
+    char* Vs = smem + C::NBUF * L::BYTES;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wq = w / WK, wk = w % WK;
 
@@ -247,32 +253,30 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o, 64));
     lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    typename Ty<T>::Frag qf[KS], gf[KS];
+    typename Ty<M>::Frag qf[KS], gf[KS];
+    float de = 0.f;                              // delta of the row, from its output and gradient
+    const T* op = static_cast<const T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h;
     const T* qp = static_cast<const T*>(a.q) + n * a.sq.n + i * a.sq.s + head * a.sq.h;
     const T* gp = static_cast<const T*>(a.dout) + n * a.sdo.n + i * a.sdo.s + head * a.sdo.h;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        qf[ks] = load_frag<VEC>(qp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
-        gf[ks] = load_frag<VEC>(gp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
+        const int left = live ? a.dh - 16 * ks - 8 * h : 0;
+        const auto gr = load_frag<VEC>(gp + 16 * ks + 8 * h, left), orow = load_frag<VEC>(op + 16 * ks + 8 * h, left);
+        qf[ks] = As<M>::frag(load_frag<VEC>(qp + 16 * ks + 8 * h, left));
+        gf[ks] = As<M>::frag(gr);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) de = fmaf((float)orow[e], (float)gr[e], de);
     }
-    float m = NAT ? 0.f : INFINITY, rl = 0.f, de = 0.f;                          // bf16: m = log2(l e^m), no separate 1 / l
+    de += __shfl_xor(de, 32, 64);
+    // kept for the dK / dV pass if that one follows
+    if (a.keep_delta && live && h == 0 && wk == 0 && sp == 0) a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h] = de;
+    float m = NAT ? 0.f : INFINITY, rl = 0.f;                          // bf16: m = log2(l e^m), no separate 1 / l
     if (live) {
         const int64_t x = (n * a.H + head) * a.Sq + i;
         m = a.row_max[x];
         rl = a.row_sum[x];
         if (NAT) rl = 1.f / rl;
         else m = m * LOG2E + __builtin_amdgcn_logf(rl);
-    }
-    {   // delta of the row, from its output and gradient; kept for the dK / dV pass if that one follows
-        const T* op = static_cast<const T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const typename Ty<T>::Frag of = load_frag<VEC>(op + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) de = fmaf((float)of[e], (float)gf[ks][e], de);
-        }
-        de += __shfl_xor(de, 32, 64);
-        if (a.keep_delta && live && h == 0 && wk == 0 && sp == 0) a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h] = de;
     }
     int begin = sp * a.per_split, stop = min(a.Sk, begin + a.per_split);
     if (a.causal) {
@@ -319,12 +323,12 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
                 all = all && (KT < 64 ? (uint32_t)bits[x] == ~0u : bits[x] == ~0ull);
             }
             if (all) {
-                sk.store(Ks + buf * KT * PITCH);
-                sv.store(Vs + buf * KT * PITCH);
+                sk.template store<L>(Ks + buf * L::BYTES);
+                sv.template store<L>(Vs + buf * L::BYTES);
             } else {
                 auto keep = [&](int r) { return (bits[WORDS > 1 ? r >> 6 : 0] >> (r & 63)) & 1; };
-                sk.store_if(Ks + buf * KT * PITCH, keep);
-                sv.store_if(Vs + buf * KT * PITCH, keep);
+                sk.template store_if<L>(Ks + buf * L::BYTES, keep);
+                sv.template store_if<L>(Vs + buf * L::BYTES, keep);
             }
         };
         const int tiles = (end - begin + KT - 1) / KT;
@@ -333,8 +337,8 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
             fetch(j0 + KT);
-            const T* Kt = Ks + buf * KT * PITCH;
-            const T* Vt = Vs + buf * KT * PITCH;
+            const char* Kt = Ks + buf * L::BYTES;
+            const char* Vt = Vs + buf * L::BYTES;
             const uint64_t mine = kb.at(j0 + 32 * wk * KSUB);
 #pragma unroll
             for (int s = 0; s < KSUB; ++s) {
@@ -342,12 +346,10 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
                 uint32_t sub = (uint32_t)(mine >> (32 * s));
                 if (!sub && !(a.additive && kw < end)) continue;
                 f32x16 x = zero16(), dp = zero16();
-                const T* kr = Kt + (ko + l31) * PITCH + 8 * h;
-                const T* vr = Vt + (ko + l31) * PITCH + 8 * h;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    x = mul(near_frag(kr + 16 * ks), qf[ks], x);
-                    dp = mul(near_frag(vr + 16 * ks), gf[ks], dp);
+                    x = mul(L::near(Kt, ko + l31, 16 * ks + 8 * h), qf[ks], x);
+                    dp = mul(L::near(Vt, ko + l31, 16 * ks + 8 * h), gf[ks], dp);
                 }
                 if (NAT) {
 #pragma unroll
@@ -374,9 +376,9 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
                 }
 #pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) {
-                    const typename Ty<T>::Frag sf = tile_frag<T>(dp, k2);
+                    const typename Ty<M>::Frag sf = tile_frag<M>(dp, k2);
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) dq[d] = mul(col_frag<PITCH>(Kt, ko + 16 * k2, 32 * d, lane), sf, dq[d]);
+                    for (int d = 0; d < DT; ++d) dq[d] = mul(L::col(Kt, ko + 16 * k2, 32 * d, lane), sf, dq[d]);
                 }
             }
             if (C::NBUF == 1) __syncthreads();

@@ -35,6 +35,10 @@ struct Args {
     int splits, per_split;
 };
 
+// what tensors of type T are multiplied as: fp32 in three parts, except with WK = 4 (few rows: bound by memory and latency)
+template <class T, int WK> struct MulType { typedef T M; };
+template <> struct MulType<float, 1> { typedef Split3 M; };
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NEVER = -1e30f;                 // running maximum before the first key: finite, so exp2(-inf - NEVER) = 0 and no inf - inf
 
@@ -84,7 +88,7 @@ __device__ __forceinline__ uint32_t keep4(const Args& a, uint64_t idx) {
 // 32-bit offset per thread (the host checks that a tile's offsets fit); otherwise element by element.
 template <class T, int DHP, int ROWS, bool VEC, int NT = 256>
 struct Stage {
-    static constexpr int E = Ty<T>::E, PITCH = DHP + Ty<T>::PAD, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / NT, STEP = NT / PER_ROW;
+    static constexpr int E = Ty<T>::E, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / NT, STEP = NT / PER_ROW;
     static_assert(ROWS * PER_ROW % NT == 0 && NT % PER_ROW == 0, "whole pieces per thread, whole rows per pass");
     u32x4 r[NCH];
     int row, col;
@@ -110,14 +114,13 @@ struct Stage {
                 r[u] = load16<T, false>(base + (int64_t)(row + STEP * u) * stride + col, row + STEP * u < rows ? dh - col : 0);
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    template <class L> __device__ __forceinline__ void store(char* lds) const {              // L: the tile's layout (mma.h)
 #pragma unroll
-        for (int u = 0; u < NCH; ++u) *reinterpret_cast<u32x4*>(lds + (row + STEP * u) * PITCH + col) = r[u];
+        for (int u = 0; u < NCH; ++u) L::put(lds, row + STEP * u, col, r[u]);
     }
-    template <class F> __device__ __forceinline__ void store_if(T* lds, F keep) const {
+    template <class L, class F> __device__ __forceinline__ void store_if(char* lds, F keep) const {
 #pragma unroll
-        for (int u = 0; u < NCH; ++u)
-            *reinterpret_cast<u32x4*>(lds + (row + STEP * u) * PITCH + col) = keep(row + STEP * u) ? r[u] : u32x4{0, 0, 0, 0};
+        for (int u = 0; u < NCH; ++u) L::put(lds, row + STEP * u, col, keep(row + STEP * u) ? r[u] : u32x4{0, 0, 0, 0});
     }
 };
 

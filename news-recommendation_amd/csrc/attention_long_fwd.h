@@ -25,9 +25,10 @@ namespace al {
 template <class T, int DHP, int WK> struct FwdCfg {
     static constexpr int KSUB = (sizeof(T) == 2 && WK == 1) ? 2 : 1;     // 32-key pieces of a tile per wave
     static constexpr int KT = 32 * KSUB * WK;
-    static constexpr int PITCH = DHP + Ty<T>::PAD;
+    typedef typename MulType<T, WK>::M M;
+    typedef Lds<M, KT, DHP> L;
     static constexpr int NBUF = (sizeof(T) == 4 && DHP == 128 && WK == 4) ? 1 : 2;       // two stages where 160 KB hold them
-    static constexpr size_t TILES = (size_t)NBUF * 2 * KT * PITCH * sizeof(T);
+    static constexpr size_t TILES = NBUF * 2 * L::BYTES;
     static constexpr size_t JOIN = WK > 1 ? (size_t)(WK * DHP * 32 + 2 * WK * 32) * 4 : 0;
     static constexpr size_t BITS = TILES > JOIN ? TILES : JOIN;          // offset of the key bits
     static constexpr size_t BYTES = BITS + SPAN / 8;
@@ -37,15 +38,17 @@ template <class T, int DHP, int WK> struct FwdCfg {
 template <class T, int DHP, bool VEC, int WK, bool DROP>
 __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_kernel(const Args a) {
     typedef FwdCfg<T, DHP, WK> C;
-    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, PITCH = C::PITCH, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
+    constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
     constexpr bool NAT = sizeof(T) == 4;         // fp32: exp(x - m) with the difference formed first (the mask's -1e5 would cost
                                                  // a product's rounding); bf16: one fma per score in units of log 2
     // the maximum may lag behind by this much before the sums are rescaled (bf16: probabilities up to 2^8, no precision is lost
     // in a floating format; the rescaling of every row's sums becomes rare)
     constexpr float SLACK = NAT ? 0.f : 8.f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + C::NBUF * KT * PITCH;
+    typedef typename C::M M;
+    typedef typename C::L L;
+    char* Ks = smem;
+    char* Vs = smem + C::NBUF * L::BYTES;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wq = w / WK, wk = w % WK;
 
@@ -63,10 +66,10 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o, 64));
     lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    typename Ty<T>::Frag qf[KS];
+    typename Ty<M>::Frag qf[KS];
     const T* qp = static_cast<const T*>(a.q) + n * a.sq.n + i * a.sq.s + head * a.sq.h;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<VEC>(qp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0);
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = As<M>::frag(load_frag<VEC>(qp + 16 * ks + 8 * h, live ? a.dh - 16 * ks - 8 * h : 0));
 
     // keys of this block
     int begin = sp * a.per_split, stop = min(a.Sk, begin + a.per_split);
@@ -117,12 +120,12 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
                 all = all && (KT < 64 ? (uint32_t)bits[x] == ~0u : bits[x] == ~0ull);
             }
             if (all) {
-                sk.store(Ks + buf * KT * PITCH);
-                sv.store(Vs + buf * KT * PITCH);
+                sk.template store<L>(Ks + buf * L::BYTES);
+                sv.template store<L>(Vs + buf * L::BYTES);
             } else {
                 auto keep = [&](int r) { return (bits[WORDS > 1 ? r >> 6 : 0] >> (r & 63)) & 1; };
-                sk.store_if(Ks + buf * KT * PITCH, keep);
-                sv.store_if(Vs + buf * KT * PITCH, keep);
+                sk.template store_if<L>(Ks + buf * L::BYTES, keep);
+                sv.template store_if<L>(Vs + buf * L::BYTES, keep);
             }
         };
         const int tiles = (end - begin + KT - 1) / KT;
@@ -131,8 +134,8 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
             fetch(j0 + KT);                      // (past the end: zeros, no memory is read)
-            const T* Kt = Ks + buf * KT * PITCH;
-            const T* Vt = Vs + buf * KT * PITCH;
+            const char* Kt = Ks + buf * L::BYTES;
+            const char* Vt = Vs + buf * L::BYTES;
             const int kw = j0 + 32 * wk * KSUB;                          // first key of this wave's piece
             const uint64_t mine = kb.at(kw);
             uint32_t sub[KSUB], any = 0, all = ~0u;
@@ -146,9 +149,8 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
 #pragma unroll
                 for (int s = 0; s < KSUB; ++s) {
                     x[s] = zero16();
-                    const T* kr = Kt + (32 * (wk * KSUB + s) + l31) * PITCH + 8 * h;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) x[s] = mul(near_frag(kr + 16 * ks), qf[ks], x[s]);
+                    for (int ks = 0; ks < KS; ++ks) x[s] = mul(L::near(Kt, 32 * (wk * KSUB + s) + l31, 16 * ks + 8 * h), qf[ks], x[s]);
                 }
                 if (NAT) {
 #pragma unroll
@@ -206,10 +208,10 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
                 for (int s = 0; s < KSUB; ++s)
 #pragma unroll
                     for (int k2 = 0; k2 < 2; ++k2) {
-                        const typename Ty<T>::Frag pf = tile_frag<T>(x[s], k2);
+                        const typename Ty<M>::Frag pf = tile_frag<M>(x[s], k2);
 #pragma unroll
                         for (int d = 0; d < DT; ++d)
-                            o[d] = mul(col_frag<PITCH>(Vt, 32 * (wk * KSUB + s) + 16 * k2, 32 * d, lane), pf, o[d]);
+                            o[d] = mul(L::col(Vt, 32 * (wk * KSUB + s) + 16 * k2, 32 * d, lane), pf, o[d]);
                     }
             }
             if (C::NBUF == 1) __syncthreads();

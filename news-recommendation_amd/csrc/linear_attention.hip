@@ -137,6 +137,8 @@ template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
     // two sets where they take at most 48 registers each, otherwise one
     static constexpr bool DEEP = ((OUT ? 2 : 1) * DA + DB) * C * (int)sizeof(T) <= 48 * 4 * NT;
     static constexpr size_t LDS = ((OUT ? 2 : 1) * PA + PB) * C * sizeof(T) + C * 4;
+    typedef Lds<T, C, DA> LA;
+    typedef Lds<T, C, DB> LB;
     struct Set {
         al::Stage<T, DA, C, VEC, NT> x, y;
         al::Stage<T, DB, C, VEC, NT> z;
@@ -173,9 +175,9 @@ template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
     __device__ __forceinline__ int put(const Set& s, int t, int tid) {
         const int m = min(C, at.s1 - at.s0 - C * tile(t));
         __syncthreads();
-        if (OUT) s.x.store(Xs);
-        s.y.store(Ys);
-        s.z.store(Zs);
+        if (OUT) s.x.template store<LA>(reinterpret_cast<char*>(Xs));
+        s.y.template store<LA>(reinterpret_cast<char*>(Ys));
+        s.z.template store<LB>(reinterpret_cast<char*>(Zs));
         if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid & 31, min(32, max(0, m - (tid & 32))), J.rev, J.umul);
         had = m;
         __syncthreads();

@@ -8,8 +8,13 @@
 //   "near":  k = 8 h + e                        (operands read as 8 consecutive elements of a row)
 //   "tile":  k = 4 h + (e & 3) + 8 * (e >> 2)   (operands that are D tiles of an earlier product: element e of k-step kb is
 //                                                register 8 kb + e, so a D tile feeds the next product without leaving the lane)
-// bf16: one v_mfma_f32_32x32x16_bf16 per k-step.  fp32: eight v_mfma_f32_32x32x2_f32, the e-th on element e of both fragments
-// (its two k's are the halves' e-th elements); full fp32 products and sums at the fp32 matrix rate.
+// Element types M of the products:
+//   __bf16  one v_mfma_f32_32x32x16_bf16 per k-step
+//   Split3  fp32 operands as the sum of three bf16 numbers each (exact: 24 bits in three eights); of the nine partial products the six
+//           largest, smallest first, on the bf16 matrix pipe, summed in fp32.  What is left out is below 2^-23 of the product: fp32
+//           accuracy at 6 / 16 of the matrix time.  An infinite operand comes out as NaN.
+//   float   eight v_mfma_f32_32x32x2_f32, the e-th on element e of both fragments (its two k's are the halves' e-th elements); where
+//           memory or latency bounds the kernel and the split would only cost registers
 #pragma once
 #include "common.h"
 
@@ -25,7 +30,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+struct Split3 {};
+struct Frag3 { bf16x8 p[3]; };                   // largest part first
+
 template <class T> struct Ty;
+template <> struct Ty<Split3> { typedef Frag3 Frag; };
 template <> struct Ty<float> {
     typedef f32x8 Frag;
     static constexpr int E = 4;        // elements per 16 bytes
@@ -54,6 +63,40 @@ __device__ __forceinline__ f32x16 mul(const f32x8& a, const f32x8& b, f32x16 c) 
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
 }
+
+__device__ __forceinline__ f32x16 mul(const Frag3& a, const Frag3& b, f32x16 c) {
+    c = mul(a.p[2], b.p[0], c);
+    c = mul(a.p[0], b.p[2], c);
+    c = mul(a.p[1], b.p[1], c);
+    c = mul(a.p[1], b.p[0], c);
+    c = mul(a.p[0], b.p[1], c);
+    return mul(a.p[0], b.p[0], c);
+}
+// two floats -> their three parts, packed in pairs (x in the low halves)
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    p0 = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+    p1 = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+    p2 = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+__device__ __forceinline__ Frag3 split8(const f32x8& v) {
+    u32x4 a, b, c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t x, y, z;
+        split_pair(v[2 * e], v[2 * e + 1], x, y, z);
+        a[e] = x; b[e] = y; c[e] = z;
+    }
+    return Frag3{{__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, c)}};
+}
+// a fragment as loaded from memory -> as multiplied
+template <class M> struct As;
+template <> struct As<__bf16> { static __device__ __forceinline__ bf16x8 frag(const bf16x8& v) { return v; } };
+template <> struct As<float> { static __device__ __forceinline__ f32x8 frag(const f32x8& v) { return v; } };
+template <> struct As<Split3> { static __device__ __forceinline__ Frag3 frag(const f32x8& v) { return split8(v); } };
 
 // 8 consecutive elements of an LDS row ("near" order: p already points at column 16 * kstep + 8 * h)
 __device__ __forceinline__ bf16x8 near_frag(const __bf16* p) { return *reinterpret_cast<const bf16x8*>(p); }
@@ -92,6 +135,47 @@ template <class T> __device__ __forceinline__ typename Ty<T>::Frag tile_frag(con
     for (int e = 0; e < 8; ++e) o[e] = (T)t[8 * kb + e];
     return o;
 }
+
+template <> __device__ __forceinline__ Frag3 tile_frag<Split3>(const f32x16& t, int kb) {
+    return split8(f32x8{t[8 * kb], t[8 * kb + 1], t[8 * kb + 2], t[8 * kb + 3], t[8 * kb + 4], t[8 * kb + 5], t[8 * kb + 6], t[8 * kb + 7]});
+}
+
+// A [ROWS x D] tile in LDS, to be multiplied as M.  put: 16 bytes of a row as they come from memory
+template <class M, int ROWS, int D> struct Lds {
+    static constexpr int PITCH = D + Ty<M>::PAD;
+    static constexpr size_t BYTES = (size_t)ROWS * PITCH * sizeof(M);
+    static __device__ __forceinline__ void put(char* t, int row, int col, const u32x4& v) {
+        *reinterpret_cast<u32x4*>(reinterpret_cast<M*>(t) + row * PITCH + col) = v;
+    }
+    static __device__ __forceinline__ typename Ty<M>::Frag near(const char* t, int row, int col) {
+        return near_frag(reinterpret_cast<const M*>(t) + row * PITCH + col);
+    }
+    static __device__ __forceinline__ typename Ty<M>::Frag col(const char* t, int row0, int col0, int lane) {
+        return col_frag<PITCH>(reinterpret_cast<const M*>(t), row0, col0, lane);
+    }
+};
+// the three parts as three bf16 tiles
+template <int ROWS, int D> struct Lds<Split3, ROWS, D> {
+    typedef Lds<__bf16, ROWS, D> L;
+    static constexpr int PITCH = L::PITCH;
+    static constexpr size_t BYTES = 3 * L::BYTES;
+    static __device__ __forceinline__ void put(char* t, int row, int col, const u32x4& v) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        uint32_t a, b, c, d, e, f;
+        split_pair(__uint_as_float(v[0]), __uint_as_float(v[1]), a, b, c);
+        split_pair(__uint_as_float(v[2]), __uint_as_float(v[3]), d, e, f);
+        char* p = t + (row * PITCH + col) * 2;
+        *reinterpret_cast<u32x2*>(p) = u32x2{a, d};
+        *reinterpret_cast<u32x2*>(p + L::BYTES) = u32x2{b, e};
+        *reinterpret_cast<u32x2*>(p + 2 * L::BYTES) = u32x2{c, f};
+    }
+    static __device__ __forceinline__ Frag3 near(const char* t, int row, int col) {
+        return Frag3{{L::near(t, row, col), L::near(t + L::BYTES, row, col), L::near(t + 2 * L::BYTES, row, col)}};
+    }
+    static __device__ __forceinline__ Frag3 col(const char* t, int row0, int col0, int lane) {
+        return Frag3{{L::col(t, row0, col0, lane), L::col(t + L::BYTES, row0, col0, lane), L::col(t + 2 * L::BYTES, row0, col0, lane)}};
+    }
+};
 
 // E consecutive elements of a global row as one 16-byte word; elements at and past `n` are zero.  VEC: the address is a multiple
 // of 16 and n is a multiple of E.
