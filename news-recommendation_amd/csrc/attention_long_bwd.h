@@ -224,11 +224,13 @@ template <class T, int DHP, int WK> struct DqCfg {
     static constexpr int NBUF = (sizeof(T) == 4 && DHP == 128 && WK == 4) ? 1 : 2;
     static constexpr size_t TILES = NBUF * 2 * L::BYTES;
     static constexpr size_t JOIN = WK > 1 ? (size_t)WK * DHP * 32 * 4 : 0;
-    static constexpr size_t BITS = TILES > JOIN ? TILES : JOIN, BYTES = BITS + SPAN / 8;
+    static constexpr size_t BITS = TILES > JOIN ? TILES : JOIN, RED = BITS + SPAN / 8, BYTES = RED + (WK > 1 ? WK * 32 * 4 : 0);
     static constexpr int WAVES = BYTES <= 80 * 1024 && DHP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1;
 };
 
-template <class T, int DHP, bool VEC, int WK, bool DROP>
+// WHOLE: all keys fit one tile (kernels of their own: in the same ones the few lines cost the long case its registers, 150 -> 241 us
+// for 4001 x 128 causal)
+template <class T, int DHP, bool VEC, int WK, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kernel(const Args a) {
     typedef DqCfg<T, DHP, WK> C;
     constexpr int WQ = 4 / WK, KSUB = C::KSUB, KT = C::KT, KS = DHP / 16, DT = DHP / 32, WORDS = (KT + 63) / 64;
@@ -334,6 +336,58 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
         const int tiles = (end - begin + KT - 1) / KT;
         if (tiles > 0) put(0, begin);
         __syncthreads();
+        // the scores and dP of 32 keys; false if none of them is there
+        auto scores = [&](const char* Kt, const char* Vt, int j0, uint64_t mine, int s, f32x16& x, f32x16& dp) {
+            const int ko = 32 * (wk * KSUB + s), kw = j0 + ko;
+            uint32_t sub = (uint32_t)(mine >> (32 * s));
+            if (!sub && !(a.additive && kw < end)) return false;
+            x = zero16(); dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                x = mul(L::near(Kt, ko + l31, 16 * ks + 8 * h), qf[ks], x);
+                dp = mul(L::near(Vt, ko + l31, 16 * ks + 8 * h), gf[ks], dp);
+            }
+            if (NAT) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] *= a.scale;
+                if (a.additive) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) if (!((sub >> tile_row(r, h)) & 1)) x[r] += a.fill;
+                    sub = (uint32_t)kb.range(kw);
+                }
+            }
+            if (sub != ~0u || kw + 31 > lim_min) hide(x, sub, kw, lim, lim_min, h);
+            return true;
+        };
+        if (WHOLE && tiles > 0) {
+            // all of the row's keys are in this tile: delta = sum_j P dP, without the stored output's rounding.  (Among few keys dP and
+            // delta are near each other: with 2 keys the bf16 output's rounding alone put dQ off by 4.4e-3 of its norm, 1.9e-3 so.)
+            float sum = 0.f;
+#pragma unroll 1
+            for (int s = 0; s < KSUB; ++s) {
+                f32x16 x, dp;
+                if (!scores(Ks, Vs, begin, kb.at(begin + 32 * wk * KSUB), s, x, dp)) continue;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t kp4 = 0xf;
+                    if (DROP) kp4 = keep4(a, ((uint64_t)(n * a.H + head) * a.Sq + i) * a.Sk + begin + 32 * (wk * KSUB + s) + 8 * q + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!DROP || ((kp4 >> e) & 1)) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(x[4 * q + e], scale2, -m)), DROP ? dp[4 * q + e] * a.keep : dp[4 * q + e], sum);
+                }
+            }
+            sum += __shfl_xor(sum, 32, 64);
+            if (WK > 1) {
+                float* red = reinterpret_cast<float*>(smem + C::RED);
+                if (h == 0) red[wk * 32 + l31] = sum;
+                __syncthreads();
+                sum = 0.f;
+#pragma unroll
+                for (int y = 0; y < WK; ++y) sum += red[y * 32 + l31];
+            }
+            de = sum;
+            if (a.keep_delta && live && h == 0 && wk == 0) a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h] = de;
+        }
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
             fetch(j0 + KT);
@@ -343,24 +397,8 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
 #pragma unroll
             for (int s = 0; s < KSUB; ++s) {
                 const int ko = 32 * (wk * KSUB + s), kw = j0 + ko;
-                uint32_t sub = (uint32_t)(mine >> (32 * s));
-                if (!sub && !(a.additive && kw < end)) continue;
-                f32x16 x = zero16(), dp = zero16();
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    x = mul(L::near(Kt, ko + l31, 16 * ks + 8 * h), qf[ks], x);
-                    dp = mul(L::near(Vt, ko + l31, 16 * ks + 8 * h), gf[ks], dp);
-                }
-                if (NAT) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] *= a.scale;
-                    if (a.additive) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) if (!((sub >> tile_row(r, h)) & 1)) x[r] += a.fill;
-                        sub = (uint32_t)kb.range(kw);
-                    }
-                }
-                if (sub != ~0u || kw + 31 > lim_min) hide(x, sub, kw, lim, h);
+                f32x16 x, dp;
+                if (!scores(Kt, Vt, j0, mine, s, x, dp)) continue;
                 const uint64_t rlin = ((uint64_t)(n * a.H + head) * a.Sq + i) * a.Sk;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -467,11 +505,15 @@ static int launch_dkv(const Args& a, unsigned grid, hipStream_t s) {
 }
 template <class T, int DHP, bool VEC, int WK, bool DROP>
 static int launch_dq(const Args& a, unsigned grid, hipStream_t s) {
-    constexpr size_t bytes = DqCfg<T, DHP, WK>::BYTES;
-    if (bytes > 64 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_dq_kernel<T, DHP, VEC, WK, DROP>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    hipLaunchKernelGGL((attn_dq_kernel<T, DHP, VEC, WK, DROP>), dim3(grid), dim3(256), bytes, s, a);
-    return check_launch("attention_bwd dq");
+    typedef DqCfg<T, DHP, WK> C;
+    auto go = [&](auto kernel) {
+        if (C::BYTES > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::BYTES);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), C::BYTES, s, a);
+        return check_launch("attention_bwd dq");
+    };
+    if constexpr (sizeof(T) == 2)                // (fp32: the output's rounding does not matter)
+        if (a.splits == 1 && a.Sk <= C::KT) return go(&attn_dq_kernel<T, DHP, VEC, WK, DROP, true>);
+    return go(&attn_dq_kernel<T, DHP, VEC, WK, DROP, false>);
 }
 template <class T, bool VEC, bool DROP> static int pick_dkv(const Args& a, unsigned grid, hipStream_t s) {
     if (a.dh <= 32) return launch_dkv<T, 32, VEC, DROP>(a, grid, s);

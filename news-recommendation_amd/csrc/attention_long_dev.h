@@ -161,13 +161,21 @@ struct KeyBits {
     }
 };
 
-// scores of this lane's row, 16 keys of 32 from key0 on: what the row must not see becomes -inf
-__device__ __forceinline__ void hide(f32x16& x, uint32_t bits, int key0, int lim, int h) {
-    if (lim - key0 < 31) bits = lim < key0 ? 0 : bits & ((2u << (lim - key0)) - 1);
-    bits >>= 4 * h;
+// scores of this lane's row, 16 keys of 32 from key0 on: what the row must not see becomes -inf.  The keys that are not there are the
+// same for every row: one wave-wide select per register; the causal end is the lane's own.
+__device__ __forceinline__ void hide(f32x16& x, uint32_t bits, int key0, int lim, int lim_min, int h) {
+    if (bits != ~0u)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (!((bits >> tile_row(r, 0)) & 1)) x[r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+            const int t = tile_row(r, 0);
+            const uint64_t on = ((bits >> t) & 1 ? 0xffffffffull : 0) | ((bits >> (t + 4)) & 1 ? 0xffffffffull << 32 : 0);
+            x[r] = __builtin_amdgcn_inverse_ballot_w64(on) ? x[r] : -INFINITY;
+        }
+    if (key0 + 31 > lim_min) {
+        const int last = lim - key0 - 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = tile_row(r, 0) <= last ? x[r] : -INFINITY;
+    }
 }
 
 // host side
