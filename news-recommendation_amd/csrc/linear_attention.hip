@@ -131,12 +131,10 @@ __device__ __forceinline__ float add_weight(float a2, int i, int m, int rev, flo
     return i < m ? umul * power(a2, rev ? i + 1 : m - 1 - i) : 0.f;
 }
 
-// the tiles of C tokens that a workgroup walks, one or two of them on their way from memory at any time
+// the tiles of C tokens that a workgroup walks, the next one on its way from memory while one is worked on
 template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
     static constexpr int NT = 2 * DB, PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, C = TILE<T>;
-    // two sets where they take at most 48 registers each, otherwise one
-    static constexpr bool DEEP = ((OUT ? 2 : 1) * DA + DB) * C * (int)sizeof(T) <= 48 * 4 * NT;
-    static constexpr size_t LDS = ((OUT ? 2 : 1) * PA + PB) * C * sizeof(T) + C * 4;
+    static constexpr size_t LDS = ((OUT ? 2 : 1) * PA + PB) * C * sizeof(T) + C * 4 + (OUT ? 64 * 4 : 0);
     typedef Lds<T, C, DA> LA;
     typedef Lds<T, C, DB> LB;
     struct Set {
@@ -200,7 +198,7 @@ __device__ __forceinline__ void absorb(f32x16 (&S)[AT], const T* Ys, const float
 }
 
 template <class T, int DA, int DB, bool VEC>
-__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_state_kernel(const Args a) {
+__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T) <= 256 && sizeof(T) == 4 ? 2 : 1))) void lin_state_kernel(const Args a) {
     constexpr int AT = DA / 32;
     typedef Walk<T, DA, DB, VEC, false> W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -211,12 +209,12 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_s
     f32x16 S[AT];
 #pragma unroll
     for (int t = 0; t < AT; ++t) S[t] = zero16();
-    typename W::Set s0, s1;
-    walk.setup(s0, tid);
-    walk.setup(s1, tid);
-    auto step = [&](typename W::Set& set, int t) {
+    typename W::Set set;
+    walk.setup(set, tid);
+    walk.fetch(set, 0);
+    for (int t = 0; t < walk.nc; ++t) {
         const int m = walk.put(set, t, tid);
-        walk.fetch(set, t + (W::DEEP ? 2 : 1));
+        walk.fetch(set, t + 1);
 #pragma unroll
         for (int u = 0; u < W::C / 32; ++u) {
             const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
@@ -226,16 +224,7 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_s
             for (int kb = 0; kb < 2; ++kb) zf[kb] = col_frag<W::PB>(walk.Zs, 32 * it + 16 * kb, 32 * w, lane);
             absorb<T, W::PA, AT, 3>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
         }
-    };
-    walk.fetch(s0, 0);
-    if (W::DEEP) {
-        walk.fetch(s1, 1);
-        for (int t = 0; t < walk.nc; t += 2) {
-            step(s0, t);
-            if (t + 1 < walk.nc) step(s1, t + 1);
-        }
-    } else
-        for (int t = 0; t < walk.nc; ++t) step(s0, t);
+    }
     float* dst = J.seg + (at.nh * a.G + at.seg) * (int64_t)(J.da * J.db);
     const int b = 32 * w + l31;
     if (b < J.db)
@@ -275,7 +264,7 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(const Args a) {
 
 // EXACT: one segment whose final state is wanted
 template <class T, int DA, int DB, bool VEC, bool EXACT>
-__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_out_kernel(const Args a) {
+__global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T) <= 256 && sizeof(T) == 4 ? 2 : 1))) void lin_out_kernel(const Args a) {
     constexpr int NT = 2 * DB, AT = DA / 32, KA = DA / 16;
     typedef Walk<T, DA, DB, VEC, true> W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -286,11 +275,9 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_o
     T* op = static_cast<T*>(J.o) + at.n * J.so.n + at.h * J.so.h;
     const int b = 32 * w + l31;
     const int64_t E = (int64_t)J.da * J.db;
-    typename W::Set set0, set1;
-    walk.setup(set0, tid);
-    walk.setup(set1, tid);
-    walk.fetch(set0, 0);
-    if (W::DEEP) walk.fetch(set1, 1);
+    typename W::Set set;
+    walk.setup(set, tid);
+    walk.fetch(set, 0);
 
     f32x16 S[AT];
     {
@@ -304,15 +291,17 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_o
                 S[x][r] = src && row < J.da && b < J.db ? src[turned ? b * J.da + row : row * J.db + b] : 0.f;
             }
     }
-    f32x16 near;                                 // decays between 32 tokens: row j, column i = l31
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int d = J.rev ? tile_row(r, h) - l31 : l31 - tile_row(r, h);
-        near[r] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
+    // decays between 32 tokens, by (row j) - (column i) + 31; zero on the side that the sum leaves out.  (In registers they took the
+    // sixteen that a third wave per SIMD needs.)
+    float* near = walk.wu + W::C;
+    if (tid < 64) {
+        const int d = J.rev ? tid - 31 : 31 - tid;
+        near[tid] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
     }
-    auto step = [&](typename W::Set& set, int t) {
+    const float* nearest = near + 31 + 4 * h - l31;
+    for (int t = 0; t < walk.nc; ++t) {
         const int t0 = at.s0 + W::C * walk.tile(t), m = walk.put(set, t, tid);
-        walk.fetch(set, t + (W::DEEP ? 2 : 1));
+        walk.fetch(set, t + 1);
 #pragma unroll 1
         for (int u = 0; u < W::C / 32; ++u) {
             const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
@@ -328,7 +317,7 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_o
                 for (int k2 = 0; k2 < 2; ++k2) o = mul(tile_frag<T>(S[y], k2), spread_frag(xr + 32 * y + 16 * k2 + 4 * h), o);
             const float wi = J.imul * power(at.a2, J.rev ? max(mi - 1 - l31, 0) : l31 + 1);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { o[r] *= wi; x[r] *= near[r]; }
+            for (int r = 0; r < 16; ++r) { o[r] *= wi; x[r] *= nearest[tile_row(r, 0)]; }
             typename Ty<T>::Frag zf[2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
@@ -345,14 +334,7 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 2 : 1)) void lin_o
             }
             absorb<T, W::PA, AT, (EXACT ? 3 : 2)>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
         }
-    };
-    if (W::DEEP)
-        for (int t = 0; t < walk.nc; t += 2) {
-            step(set0, t);
-            if (t + 1 < walk.nc) step(set1, t + 1);
-        }
-    else
-        for (int t = 0; t < walk.nc; ++t) step(set0, t);
+    }
     if (EXACT && J.last && b < J.db)
 #pragma unroll
         for (int x = 0; x < AT; ++x)
@@ -413,12 +395,13 @@ __global__ __launch_bounds__(256) void lin_step_kernel(const T* __restrict__ q, 
 }
 
 // ---------------------------------------------------------------- host
-// heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each
+// heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each, at least three of them: the extra
+// pass reads y and z again (32 x 12 heads of 1000 x 64: 76 us whole, 81 us in two; 2 x 12 of 16384: 88 us in 37)
 static void cut(Args& a) {
     const int64_t blocks = a.jobs * a.N * a.H;
     a.G = 1; a.per = (a.S + UNIT - 1) / UNIT * UNIT;
     const int64_t want = std::min<int64_t>(blocks > 0 ? 1024 / blocks : 0, a.S / 256);
-    if (want < 2) return;
+    if (want < 3) return;
     a.per = (int)((((int64_t)a.S + want - 1) / want + UNIT - 1) / UNIT * UNIT);
     a.G = (a.S + a.per - 1) / a.per;
 }
