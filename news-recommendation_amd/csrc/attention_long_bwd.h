@@ -103,8 +103,8 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
     float st[3];
     auto fetch = [&](int hh, int i0, bool any) {
         const int head = g * a.rep + hh, rows = any ? a.Sq - i0 : 0;
-        sq.load(static_cast<const T*>(a.q) + n * a.sq.n + i0 * a.sq.s + head * a.sq.h, a.sq.s, rows, a.dh);
-        sg.load(static_cast<const T*>(a.dout) + n * a.sdo.n + i0 * a.sdo.s + head * a.sdo.h, a.sdo.s, rows, a.dh);
+        sq.load(static_cast<const T*>(a.q) + n * a.sq.n + i0 * a.sq.s + head * a.sq.h, rows);
+        sg.load(static_cast<const T*>(a.dout) + n * a.sdo.n + i0 * a.sdo.s + head * a.sdo.h, rows);
         if (tid < QT) {
             st[0] = 0.f; st[1] = INFINITY; st[2] = 0.f;                          // (no row: its probabilities come out as zero)
             if (tid < rows) {
@@ -302,13 +302,19 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
     kb.words = reinterpret_cast<uint64_t*>(smem + C::BITS);
     kb.masked = mask != nullptr;
     int end = stop;
-    auto fetch = [&](int j) {
-        sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
-        sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
+    const T *kn = nullptr, *vn = nullptr;        // the next tile
+    const int64_t kstep = KT * a.sk.s, vstep = KT * a.sv.s;
+    auto fetch = [&](int left) {                 // (none left: zeros, no memory is read)
+        sk.load(kn, left);
+        sv.load(vn, left);
+        kn += kstep;
+        vn += vstep;
     };
     for (; begin < stop; begin += SPAN) {        // (one turn without a mask)
         end = stop;
-        fetch(begin);                            // on its way while the key bits are read
+        kn = kp + begin * a.sk.s;
+        vn = vp + begin * a.sv.s;
+        fetch(end - begin);                      // on its way while the key bits are read
         kb.from = begin;
         kb.end = stop;
         if (mask) {
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
         }
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
-            fetch(j0 + KT);
+            fetch(end - j0 - KT);
             const char* Kt = Ks + buf * L::BYTES;
             const char* Vt = Vs + buf * L::BYTES;
             const uint64_t mine = kb.at(j0 + 32 * wk * KSUB);

@@ -91,27 +91,28 @@ struct Stage {
     static constexpr int E = Ty<T>::E, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / NT, STEP = NT / PER_ROW;
     static_assert(ROWS * PER_ROW % NT == 0 && NT % PER_ROW == 0, "whole pieces per thread, whole rows per pass");
     u32x4 r[NCH];
-    int row, col;
-    uint32_t voff, step;
-    __device__ __forceinline__ void setup(int tid, int64_t stride, int dh) {
+    int row, col, width, pitch;                 // this thread's first piece; columns, and elements from row to row (VEC)
+    uint32_t voff;
+    int64_t stride;
+    __device__ __forceinline__ void setup(int tid, int64_t row_stride, int columns) {
         row = tid / PER_ROW;
         col = (tid % PER_ROW) * E;
-        if (VEC) {
-            voff = col < dh ? (uint32_t)(row * (int)stride + col) * (uint32_t)sizeof(T) : 0x80000000u;
-            step = STEP * (uint32_t)stride * (uint32_t)sizeof(T);
-        }
+        width = columns;
+        stride = row_stride;
+        pitch = (int)row_stride;
+        voff = col < width ? (uint32_t)(row * pitch + col) * (uint32_t)sizeof(T) : 0x80000000u;
     }
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dh) {
+    __device__ __forceinline__ void load(const T* base, int rows) {
         if (VEC) {
-            const uint64_t bytes = rows > 0 ? ((uint64_t)(rows - 1) * (uint64_t)stride + dh) * sizeof(T) : 0;
+            const int n = rows < ROWS ? rows : ROWS;                             // (so the tile's extent fits 32 bits)
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<T*>(base), 0, (int)(bytes < 0x7fffffffu ? bytes : 0x7fffffffu), 0x00020000);
+                const_cast<T*>(base), 0, n > 0 ? ((n - 1) * pitch + width) * (int)sizeof(T) : 0, 0x00020000);
 #pragma unroll
-            for (int u = 0; u < NCH; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(voff + u * step), 0, 0);
+            for (int u = 0; u < NCH; ++u) r[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(voff + u * (uint32_t)(STEP * pitch * (int)sizeof(T))), 0, 0);
         } else {
 #pragma unroll
             for (int u = 0; u < NCH; ++u)
-                r[u] = load16<T, false>(base + (int64_t)(row + STEP * u) * stride + col, row + STEP * u < rows ? dh - col : 0);
+                r[u] = load16<T, false>(base + (row + STEP * u) * stride + col, row + STEP * u < rows ? width - col : 0);
         }
     }
     template <class L> __device__ __forceinline__ void store(char* lds) const {              // L: the tile's layout (mma.h)

@@ -96,13 +96,19 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
     kb.words = reinterpret_cast<uint64_t*>(smem + C::BITS);
     kb.masked = mask != nullptr;
     int end = stop;
-    auto fetch = [&](int j) {
-        sk.load(kp + (int64_t)j * a.sk.s, a.sk.s, end - j, a.dh);
-        sv.load(vp + (int64_t)j * a.sv.s, a.sv.s, end - j, a.dh);
+    const T *kn = nullptr, *vn = nullptr;        // the next tile
+    const int64_t kstep = KT * a.sk.s, vstep = KT * a.sv.s;
+    auto fetch = [&](int left) {                 // (none left: zeros, no memory is read)
+        sk.load(kn, left);
+        sv.load(vn, left);
+        kn += kstep;
+        vn += vstep;
     };
     for (; begin < stop; begin += SPAN) {        // (one turn without a mask)
         end = stop;
-        fetch(begin);                            // on its way while the key bits are read
+        kn = kp + begin * a.sk.s;
+        vn = vp + begin * a.sv.s;
+        fetch(end - begin);                      // on its way while the key bits are read
         kb.from = begin;
         kb.end = stop;
         if (mask) {
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
             const int j0 = begin + t * KT, buf = C::NBUF == 2 ? (t & 1) : 0;
-            fetch(j0 + KT);                      // (past the end: zeros, no memory is read)
+            fetch(end - j0 - KT);
             const char* Kt = Ks + buf * L::BYTES;
             const char* Vt = Vs + buf * L::BYTES;
             const int kw = j0 + 32 * wk * KSUB;                          // first key of this wave's piece

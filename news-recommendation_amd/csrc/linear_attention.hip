@@ -142,41 +142,47 @@ template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
         al::Stage<T, DB, C, VEC, NT> z;
     };
     const Place& at;
-    const Job& J;
-    const T *xp, *yp, *zp;
+    const T *xp = nullptr, *yp, *zp;             // the next tile
+    int64_t xstep = 0, ystep, zstep;
+    int rev;
+    float umul;
     T *Xs, *Ys, *Zs;
     float* wu;
     int had = -1, nc;
-    __device__ __forceinline__ Walk(const Place& at, const Job& J, char* smem) : at(at), J(J) {
+    __device__ __forceinline__ Walk(const Place& at, const Job& J, char* smem) : at(at) {
         nc = (at.s1 - at.s0 + C - 1) / C;
-        if (OUT) xp = static_cast<const T*>(J.x) + at.n * J.sx.n + at.h * J.sx.h;
-        yp = static_cast<const T*>(J.y) + at.n * J.sy.n + at.h * J.sy.h;
-        zp = static_cast<const T*>(J.z) + at.n * J.sz.n + at.h * J.sz.h;
+        rev = J.rev; umul = J.umul;
+        const int64_t first = at.s0 + C * (rev ? nc - 1 : 0), dir = rev ? -C : C;
+        if (OUT) { xp = static_cast<const T*>(J.x) + at.n * J.sx.n + at.h * J.sx.h + first * J.sx.s; xstep = dir * J.sx.s; }
+        yp = static_cast<const T*>(J.y) + at.n * J.sy.n + at.h * J.sy.h + first * J.sy.s; ystep = dir * J.sy.s;
+        zp = static_cast<const T*>(J.z) + at.n * J.sz.n + at.h * J.sz.h + first * J.sz.s; zstep = dir * J.sz.s;
         Ys = reinterpret_cast<T*>(smem);
         Zs = Ys + C * PA;
         Xs = Zs + C * PB;
         wu = reinterpret_cast<float*>(Xs + (OUT ? C * PA : 0));
     }
-    __device__ __forceinline__ void setup(Set& s, int tid) const {
+    __device__ __forceinline__ void setup(Set& s, const Job& J, int tid) const {
         if (OUT) s.x.setup(tid, J.sx.s, J.da);
         s.y.setup(tid, J.sy.s, J.da);
         s.z.setup(tid, J.sz.s, J.db);
     }
-    __device__ __forceinline__ int tile(int t) const { return J.rev ? nc - 1 - t : t; }
-    __device__ __forceinline__ void fetch(Set& s, int t) const {                 // (past the last tile: zeros, no memory is read)
-        const int t0 = at.s0 + C * tile(t), rows = t < nc ? at.s1 - t0 : 0;
-        if (OUT) s.x.load(xp + t0 * J.sx.s, J.sx.s, rows, J.da);
-        s.y.load(yp + t0 * J.sy.s, J.sy.s, rows, J.da);
-        s.z.load(zp + t0 * J.sz.s, J.sz.s, rows, J.db);
+    __device__ __forceinline__ int tile(int t) const { return rev ? nc - 1 - t : t; }
+    __device__ __forceinline__ int tokens(int t) const { return at.s1 - at.s0 - C * tile(t); }      // from the tile's start on
+    __device__ __forceinline__ void fetch(Set& s, int t) {                       // (past the last tile: zeros, no memory is read)
+        const int rows = t < nc ? tokens(t) : 0;
+        if (OUT) s.x.load(xp, rows);
+        s.y.load(yp, rows);
+        s.z.load(zp, rows);
+        xp += xstep; yp += ystep; zp += zstep;
     }
     // tile t into LDS; returns its token count
     __device__ __forceinline__ int put(const Set& s, int t, int tid) {
-        const int m = min(C, at.s1 - at.s0 - C * tile(t));
+        const int m = min(C, tokens(t));
         __syncthreads();
         if (OUT) s.x.template store<LA>(reinterpret_cast<char*>(Xs));
         s.y.template store<LA>(reinterpret_cast<char*>(Ys));
         s.z.template store<LB>(reinterpret_cast<char*>(Zs));
-        if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid & 31, min(32, max(0, m - (tid & 32))), J.rev, J.umul);
+        if (m != had && tid < C) wu[tid] = add_weight(at.a2, tid & 31, min(32, max(0, m - (tid & 32))), rev, umul);
         had = m;
         __syncthreads();
         return m;
@@ -210,14 +216,14 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
 #pragma unroll
     for (int t = 0; t < AT; ++t) S[t] = zero16();
     typename W::Set set;
-    walk.setup(set, tid);
+    walk.setup(set, J, tid);
     walk.fetch(set, 0);
     for (int t = 0; t < walk.nc; ++t) {
         const int m = walk.put(set, t, tid);
         walk.fetch(set, t + 1);
 #pragma unroll
         for (int u = 0; u < W::C / 32; ++u) {
-            const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
+            const int it = walk.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
             if (mi <= 0) continue;
             typename Ty<T>::Frag zf[2];
 #pragma unroll
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
     const int b = 32 * w + l31;
     const int64_t E = (int64_t)J.da * J.db;
     typename W::Set set;
-    walk.setup(set, tid);
+    walk.setup(set, J, tid);
     walk.fetch(set, 0);
 
     f32x16 S[AT];
@@ -299,12 +305,15 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
         near[tid] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
     }
     const float* nearest = near + 31 + 4 * h - l31;
+    const float imul = J.imul;
+    const int64_t ostep = J.so.s;
+    const int db = J.db;
     for (int t = 0; t < walk.nc; ++t) {
         const int t0 = at.s0 + W::C * walk.tile(t), m = walk.put(set, t, tid);
         walk.fetch(set, t + 1);
 #pragma unroll 1
         for (int u = 0; u < W::C / 32; ++u) {
-            const int it = J.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
+            const int it = walk.rev ? W::C / 32 - 1 - u : u, mi = min(32, m - 32 * it);
             if (mi <= 0) continue;
             const T* xr = walk.Xs + (32 * it + l31) * W::PA;
             const T* yr = walk.Ys + (32 * it + l31) * W::PA;
@@ -315,7 +324,7 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
             for (int y = 0; y < AT; ++y)
 #pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) o = mul(tile_frag<T>(S[y], k2), spread_frag(xr + 32 * y + 16 * k2 + 4 * h), o);
-            const float wi = J.imul * power(at.a2, J.rev ? max(mi - 1 - l31, 0) : l31 + 1);
+            const float wi = imul * power(at.a2, walk.rev ? max(mi - 1 - l31, 0) : l31 + 1);
 #pragma unroll
             for (int r = 0; r < 16; ++r) { o[r] *= wi; x[r] *= nearest[tile_row(r, 0)]; }
             typename Ty<T>::Frag zf[2];
@@ -325,11 +334,11 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
                 o = mul(zf[kb], tile_frag<T>(x, kb), o);
             }
             if (l31 < mi) {
-                T* row = op + (int64_t)(t0 + 32 * it + l31) * J.so.s;
+                T* row = op + (t0 + 32 * it + l31) * ostep;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int col = 32 * w + 8 * q + 4 * h;
-                    store4<VEC>(row + col, f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]}, J.db - col);
+                    store4<VEC>(row + col, f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]}, db - col);
                 }
             }
             absorb<T, W::PA, AT, (EXACT ? 3 : 2)>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
