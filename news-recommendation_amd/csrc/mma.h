@@ -178,23 +178,29 @@ template <int ROWS, int D> struct Lds<Split3, ROWS, D> {
 };
 
 // E consecutive elements of a global row as one 16-byte word; elements at and past `n` are zero.  VEC: the address is a multiple
-// of 16 and n is a multiple of E.
+// of 16 and n is a multiple of E; otherwise the address is a multiple of the element's size: a whole word is still one load (global
+// memory takes 16-byte loads at any address), the end of a row comes element by element.
 template <class T, bool VEC>
 __device__ __forceinline__ u32x4 load16(const T* p, int n) {
+    constexpr int E = Ty<T>::E;
     if (n <= 0) return u32x4{0, 0, 0, 0};
     if (VEC) return *reinterpret_cast<const u32x4*>(p);
+    u32x4 o = {0, 0, 0, 0};
+    if (n >= E) {
+        __builtin_memcpy(&o, p, 16);
+        return o;
+    }
     if (sizeof(T) == 4) {
-        u32x4 o = {0, 0, 0, 0};
         const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (e < n) o[e] = w[e];
+        for (int e = 0; e < 3; ++e) if (e < n) o[e] = w[e];
         return o;
     }
     uint32_t s[8];
     const uint16_t* w = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = e < n ? w[e] : 0;
-    return u32x4{s[0] | s[1] << 16, s[2] | s[3] << 16, s[4] | s[5] << 16, s[6] | s[7] << 16};
+    for (int e = 0; e < 7; ++e) s[e] = e < n ? w[e] : 0;
+    return u32x4{s[0] | s[1] << 16, s[2] | s[3] << 16, s[4] | s[5] << 16, s[6]};
 }
 // a whole fragment (8 consecutive elements, "near" order) from global memory
 template <bool VEC> __device__ __forceinline__ bf16x8 load_frag(const __bf16* p, int n) {
@@ -207,15 +213,17 @@ template <bool VEC> __device__ __forceinline__ f32x8 load_frag(const float* p, i
 }
 // four consecutive elements (registers 4 i .. 4 i + 3 of a D tile whose rows run along the output's last axis)
 template <bool VEC> __device__ __forceinline__ void store4(__bf16* p, const f32x4& v, int n) {
-    bf16x4 o = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    const bf16x4 o = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
     if (VEC) { if (n > 0) *reinterpret_cast<bf16x4*>(p) = o; return; }
+    if (n >= 4) { __builtin_memcpy(p, &o, 8); return; }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (e < n) p[e] = o[e];
+    for (int e = 0; e < 3; ++e) if (e < n) p[e] = o[e];
 }
 template <bool VEC> __device__ __forceinline__ void store4(float* p, const f32x4& v, int n) {
     if (VEC) { if (n > 0) *reinterpret_cast<f32x4*>(p) = v; return; }
+    if (n >= 4) { __builtin_memcpy(p, &v, 16); return; }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (e < n) p[e] = v[e];
+    for (int e = 0; e < 3; ++e) if (e < n) p[e] = v[e];
 }
 
 }  // namespace mma

@@ -581,7 +581,7 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
         raise NewsrecError(f"attention: scale {scale} is not a positive number")
     if not 0.0 <= p_drop < 1.0:
         raise NewsrecError(f"attention: p_drop {p_drop} not in [0, 1)")
-    cfg = (1 if causal else 0, scale, float(p_drop), int(seed), int(site))
+    cfg = (1 if causal else 0, scale, float(p_drop), int(seed) & 0xFFFFFFFFFFFFFFFF, int(site) & 0xFFFFFFFF)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, key_mask, cfg)
     return _attention_fwd(q, k, v, key_mask, cfg, False)[0]

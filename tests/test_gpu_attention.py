@@ -1,6 +1,7 @@
 """ops.attention (softmax attention of any length, forward and backward) against the definition in 64 bits, with error bounds
 derived per element (attention_oracle.py), and the layers that run on it past 128 positions."""
 import math
+import random
 
 import pytest
 import torch
@@ -233,6 +234,40 @@ def test_two_graphs_do_not_share_scratch(ops):
                     g.replay()
             torch.cuda.synchronize()
             assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_problems(ops, seed):
+    """sizes, head layouts, masks, order, type and dropout drawn at random"""
+    r = random.Random(seed)
+    log = lambda hi: int(round(math.exp(r.uniform(0, math.log(hi)))))                    # noqa: E731
+    G = r.choice([1, 2, 3])
+    size = (log(4), log(300), log(600), G * r.choice([1, 2, 5]), G, r.choice([1, 3, 8, 16, 24, 25, 40, 64, 72, 96, 104, 127, 128]))
+    dtype, causal, kind, p = r.choice([F32, BF16]), r.random() < 0.4, r.choice(["none", "prefix", "holes", "last"]), r.choice([0.0, 0.0, 0.3])
+    q, k, v, do = make(seed, *size, dtype)
+    m = make_mask(kind, seed, size[0], size[2])
+    scale = r.choice([None, 0.3])
+    keep = keep_mask((size[0], size[3], size[1], size[2]), p, seed, 1) if p else None
+    want = reference(q, k, v, m, causal, scale=scale, do=do, keep=keep, p_drop=p)
+    got = run(ops, q, k, v, do, key_mask=m, causal=causal, scale=scale, p_drop=p, seed=seed, site=1)
+    for name, t in zip(("o", "dq", "dk", "dv"), got):
+        check(f"{name} {size} {dtype} causal={causal} mask={kind} p={p}", t, want[name])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size,causal", [((2, 3, 20011, 140, 140, 16), False), ((1, 40, 17000, 256, 256, 16), True)])
+@pytest.mark.parametrize("kind", ["prefix", "holes"])
+def test_masks_longer_than_one_span_of_key_bits(ops, size, causal, kind, dtype):
+    """enough heads that the keys are not split: a workgroup walks more keys than it holds presence bits for at a time"""
+    q, k, v, do = make(31, *size, dtype)
+    m = make_mask(kind, 4, size[0], size[2])
+    m[:, 9000:18000] = 0                         # a whole span without a key
+    got = run(ops, q, k, v, do, key_mask=m, causal=causal)
+    for h in range(0, size[3], 37):
+        one = [t[:, :, h:h + 1] for t in (q, k, v, do)]
+        want = reference(*one[:3], m, causal, do=one[3])
+        for name, t in zip(("o", "dq", "dk", "dv"), got):
+            check(name, t[:, :, h:h + 1], want[name])
 
 
 def test_offsets_past_32_bits(ops):

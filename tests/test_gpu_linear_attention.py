@@ -8,6 +8,7 @@ a state within (u^3 + e) M.
 e counts the fp32 arithmetic: dots of dk products, sums over S tokens (2^-24 each, worst case), a power's 2 units per chunk, and
 the argument of a power, whose error 2^-23 |a n| matters only while w^n is not zero in fp32, |a n| < 150."""
 import math
+import random
 
 import pytest
 import torch
@@ -129,6 +130,22 @@ def test_forward_and_gradients(ops, size, ragged, carried, dtype):
     with torch.no_grad():
         o, last = ops.linear_attention(t["q"], t["k"], t["v"], a, lens=lens, state=t["state"] if carried else None)
         assert torch.equal(o, got["o"]) and torch.equal(last, got["last"])
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_random_problems(ops, seed):
+    """sizes, widths, lengths, type and decays drawn at random"""
+    r = random.Random(seed)
+    log = lambda hi: int(round(math.exp(r.uniform(0, math.log(hi)))))                      # noqa: E731
+    wide = [1, 3, 8, 16, 24, 25, 40, 64, 72, 100, 128]
+    size = (log(4), log(1500), log(5), r.choice(wide), r.choice(wide))
+    dtype, carried = r.choice([F32, BF16]), r.random() < 0.5
+    t = make(seed, *size, dtype)
+    a = -torch.exp(torch.randn(size[2], generator=torch.Generator().manual_seed(seed)) * 2 - 2).cuda()
+    lens = torch.tensor([r.randint(0, size[1]) for _ in range(size[0])]).cuda() if r.random() < 0.5 else None
+    want = reference(t["q"], t["k"], t["v"], a, lens, t["state"] if carried else None, do=t["do"], dlast=t["dlast"])
+    for name, x in run(ops, t, a, lens, carried).items():
+        check(f"{name} {size} {dtype} carried={carried}", x, want[name])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
