@@ -158,11 +158,14 @@ int nr_mhsa_bwd_bf16(const void* qkv, const int64_t* mask, const void* dctx, con
  * (the reference's attention core, attention.py:87-97, without its bound on the length, for queries and keys of different
  * lengths, shared key heads and causal order).  A key j takes part if key_mask[n,j] != 0 (key_mask [N,Sk] int64, NULL: all) and,
  * with causal, j <= i + Sk - Sq: the last query stands at the last key.  A row without any key is zero and sends no gradient.
- * Rows of k / v whose mask is 0 are never used, whatever they hold; with causal order alone a later row of the same sequence
- * that is not finite can reach earlier queries of its tile (as 0 * inf).
+ * Rows of k / v whose mask is 0 are never used, whatever they hold.  Everything else has to be finite: a row that only the causal
+ * order hides can reach the queries of its tile as 0 * inf, and an infinite fp32 operand gives NaN (fp32 is multiplied as three
+ * bf16 numbers each, to fp32 accuracy).  bf16: scores scale * q.k beyond 2^16 cost the gradients accuracy (the row's maximum, in
+ * fp32, is off by half a step), beyond 2^30 the output as well.
  * q [N,Sq,H,dh], k / v [N,Sk,G,dh]: dtype 0 = fp32, 1 = bf16; innermost axis dense, the other strides in elements, any (0 as
  * well); multiples of 16 bytes throughout run faster.  out, dout, dq, dk, dv: dense, same dtype.  dh <= 128.
- * row_max / row_sum [N,H,Sq] fp32 (NULL in evaluation): the softmax statistics that the backward reuses.
+ * row_max / row_sum [N,H,Sq] fp32 (NULL in evaluation): the softmax statistics that the backward reuses (for bf16 the maximum is in
+ * units of log 2, and may lag behind the true one).
  * Dropout on the probabilities: element index ((n*H + h)*Sq + i)*Sk + j of (seed, site).
  * ws: nr_attention_{fwd,bwd}_ws_bytes(p) bytes (0 for most sizes), scratch of this call alone. */
 typedef struct {

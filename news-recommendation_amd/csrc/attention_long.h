@@ -22,7 +22,7 @@ struct AttnProblem {
 struct AttnOut {                                // what the forward writes
     void* out = nullptr;
     AttnStrides so;
-    float *row_max = nullptr, *row_sum = nullptr;      // [N,H,Sq], both or neither
+    float *row_max = nullptr, *row_sum = nullptr;      // [N,H,Sq], both or neither; the maximum of bf16 problems in units of log 2
 };
 struct AttnGrad {                               // what the backward reads besides the problem, and writes
     const void *out = nullptr, *dout = nullptr;

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
     typedef typename C::L L;
     char* Qs = smem;
     char* Gs = smem + 2 * L::BYTES;
-    float* St = reinterpret_cast<float*>(smem + C::TILES);                       // [2][3][QT]: fp32 m, 1 / l, delta; bf16 log2(l e^m), -, delta
+    float* St = reinterpret_cast<float*>(smem + C::TILES);                       // [2][3][QT]: fp32 m, 1 / l, delta; bf16 m + log2 l, -, delta
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         if (tid < QT) {
             float* s = St + buf * 3 * QT + tid;
             if (NAT) { s[0] = st[0]; s[QT] = 1.f / st[1]; }
-            else s[0] = st[0] * LOG2E + __builtin_amdgcn_logf(st[1]);
+            else s[0] = st[0] + __builtin_amdgcn_logf(st[1]);
             s[2 * QT] = st[2];
         }
     };
@@ -272,13 +272,13 @@ __global__ __launch_bounds__(256, (DqCfg<T, DHP, WK>::WAVES)) void attn_dq_kerne
     de += __shfl_xor(de, 32, 64);
     // kept for the dK / dV pass if that one follows
     if (a.keep_delta && live && h == 0 && wk == 0 && sp == 0) a.delta[n * a.sd.n + i * a.sd.s + head * a.sd.h] = de;
-    float m = NAT ? 0.f : INFINITY, rl = 0.f;                          // bf16: m = log2(l e^m), no separate 1 / l
+    float m = NAT ? 0.f : INFINITY, rl = 0.f;                          // bf16: m + log2 l, no separate 1 / l
     if (live) {
         const int64_t x = (n * a.H + head) * a.Sq + i;
         m = a.row_max[x];
         rl = a.row_sum[x];
         if (NAT) rl = 1.f / rl;
-        else m = m * LOG2E + __builtin_amdgcn_logf(rl);
+        else m += __builtin_amdgcn_logf(rl);
     }
     int begin = sp * a.per_split, stop = min(a.Sk, begin + a.per_split);
     if (a.causal) {

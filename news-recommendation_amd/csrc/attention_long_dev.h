@@ -39,8 +39,8 @@ struct Args {
 template <class T, int WK> struct MulType { typedef T M; };
 template <> struct MulType<float, 1> { typedef Split3 M; };
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float NEVER = -1e30f;                 // running maximum before the first key: finite, so exp2(-inf - NEVER) = 0 and no inf - inf
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NEVER = -3.402823466e38f;       // running maximum before the first key: finite, so exp2(-inf - NEVER) = 0 and no inf - inf
 
 // Neighbouring workgroups go to different XCDs, each with its own L2.  Key heads are dealt to the XCDs, so that the workgroups of one
 // head share an L2 and sequences of different lengths still spread over the chip; what is left of a multiple of 8 heads is spread

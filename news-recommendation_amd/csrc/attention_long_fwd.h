@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, (FwdCfg<T, DHP, WK>::WAVES)) void attn_fwd_ker
         }
     if (a.row_max && h == 0 && wk == 0) {
         const int64_t x = (n * a.H + head) * a.Sq + i;
-        a.row_max[x] = l == 0.f ? 0.f : (NAT ? m : m * LN2);
+        a.row_max[x] = l == 0.f ? 0.f : m;
         a.row_sum[x] = l == 0.f ? 1.f : l;
     }
 }
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const Args a) {
     store4<false>(static_cast<T*>(a.out) + n * a.so.n + i * a.so.s + head * a.so.h + c, o, a.dh - c);
     if (a.row_max && c == 0) {
         const int64_t x = (n * a.H + head) * a.Sq + i;
-        a.row_max[x] = l == 0.f ? 0.f : (NAT ? M : M * LN2);
+        a.row_max[x] = l == 0.f ? 0.f : M;
         a.row_sum[x] = l == 0.f ? 1.f : l;
     }
 }

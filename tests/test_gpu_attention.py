@@ -105,6 +105,25 @@ def test_masked_rows_may_hold_anything(ops, size, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("Sq", [3, 70])
+@pytest.mark.parametrize("dtype,power", [(F32, 57), (BF16, 13)], ids=["fp32", "bf16"])
+def test_scores_far_below_zero(ops, dtype, power, Sq):
+    """every score the same and far below zero (fp32: -2^117, bf16: -2^29; powers of two, so exact): every key weighs 1 / Sk"""
+    Sk, d = 300, 64
+    _, _, v, do = make(15, 2, Sq, Sk, 2, 2, d, dtype)
+    q = torch.full((2, Sq, 2, d), 2.0 ** power, device="cuda", dtype=dtype)
+    k = torch.full((2, Sk, 2, d), -2.0 ** power, device="cuda", dtype=dtype)
+    o, dq, dk, dv = run(ops, q, k, v, do)
+    # sums of n terms in fp32 (n 2^-24 of their absolute values), for bf16 the weight as an operand and the result rounded (half a step each)
+    u = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    mean = v.double().mean(1, keepdim=True).expand(2, Sq, 2, d)
+    off = (o.double() - mean).abs()
+    assert bool((off <= (u + (Sk + 8) * 2.0 ** -24) * v.double().abs().mean(1, keepdim=True) + (u + 2.0 ** -24) * mean.abs()).all())
+    if dtype == F32:
+        want = (do.double().sum(1, keepdim=True) / Sk).expand(2, Sk, 2, d)
+        assert bool(((dv.double() - want).abs() <= (Sq + 8) * 2.0 ** -24 * do.double().abs().sum(1, keepdim=True) / Sk + 2.0 ** -24 * want.abs()).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("d", [64, 25])
 def test_strided_views_and_shared_storage(ops, d, dtype):
