@@ -506,23 +506,24 @@ def _attention_problem(q, k, v, mask, causal, scale, p, seed, site):
 
 
 def _attention_fwd(q, k, v, mask, cfg, train):
-    """(out, row_max, row_sum); the statistics are None unless a backward is to follow"""
+    """(out, stats): row maximum and row sum [2,N,H,Sq], None unless a backward is to follow"""
     N, Sq, H, dh = q.shape
     out = torch.empty((N, Sq, H, dh), dtype=q.dtype, device=q.device)
     if out.numel() == 0 or k.shape[1] == 0:
-        return out.zero_(), None, None
-    rmax = rsum = ws = None
+        return out.zero_(), None
+    stats = rmax = rsum = ws = None
     if train:
-        rmax = torch.empty((N, H, Sq), dtype=torch.float32, device=q.device)
-        rsum = torch.empty((N, H, Sq), dtype=torch.float32, device=q.device)
+        stats = torch.empty((2, N, H, Sq), dtype=torch.float32, device=q.device)
+        rmax = stats.data_ptr()
+        rsum = rmax + 4 * N * H * Sq
     L = lib()
     with _on_device(q):
         P = _attention_problem(q, k, v, mask, *cfg)
         nbytes = L.nr_attention_fwd_ws_bytes(P)
         if nbytes:
             ws = _ws(nbytes, q.device)
-        check(L.nr_attention_fwd(P, out.data_ptr(), _p(rmax), _p(rsum), _p(ws), nbytes, _stream()), "nr_attention_fwd")
-    return out, rmax, rsum
+        check(L.nr_attention_fwd(P, out.data_ptr(), rmax, rsum, _p(ws), nbytes, _stream()), "nr_attention_fwd")
+    return out, stats
 
 
 class _Attention(torch.autograd.Function):
@@ -530,8 +531,8 @@ class _Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, cfg):
         ctx.set_materialize_grads(False)
         ctx.cfg = cfg
-        out, rmax, rsum = _attention_fwd(q, k, v, mask, cfg, True)
-        ctx.save_for_backward(q, k, v, mask, out if rmax is not None else None, rmax, rsum)
+        out, stats = _attention_fwd(q, k, v, mask, cfg, True)
+        ctx.save_for_backward(q, k, v, mask, None if stats is None else out, stats)
         return out
 
     @staticmethod
@@ -539,20 +540,21 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, g):
         if g is None:
             return (None,) * 5
-        q, k, v, mask, out, rmax, rsum = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        q, k, v, mask, out, stats = ctx.saved_tensors
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         if out is None:                          # an empty axis: nothing was computed, every gradient is zero
             return dq.zero_(), dk.zero_(), dv.zero_(), None, None
         g = g.contiguous()
         N, Sq, H, _ = q.shape
-        delta = torch.empty(N, H, Sq, dtype=torch.float32, device=q.device)
+        rmax = stats.data_ptr()
+        delta = torch.empty((N, H, Sq), dtype=torch.float32, device=q.device)      # (not kept with stats: two backward passes may run at once)
         L = lib()
         with _on_device(q):
             P = _attention_problem(q, k, v, mask, *ctx.cfg)
             nbytes = L.nr_attention_bwd_ws_bytes(P)
             ws = _ws(nbytes, q.device) if nbytes else None
-            check(L.nr_attention_bwd(P, _p(out), _p(g), _p(rmax), _p(rsum), _p(delta), _p(dq), _p(dk), _p(dv), _p(ws), nbytes,
-                                     _stream()), "nr_attention_bwd")
+            check(L.nr_attention_bwd(P, _p(out), _p(g), rmax, rmax + 4 * N * H * Sq, delta.data_ptr(), _p(dq), _p(dk), _p(dv),
+                                     _p(ws), nbytes, _stream()), "nr_attention_bwd")
         return dq, dk, dv, None, None
 
 
@@ -561,8 +563,10 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
     -> [N,Sq,H,dh]; fp32 or bf16, dh <= 128, any strides with a dense innermost axis (the blocks of one [N,S,3,H,dh] projection
     are read where they are).  H a multiple of G: query head h reads key head h // (H // G).  key_mask [N,Sk] 0/1 or bool: keys
     with 0 do not take part, whatever their rows hold.  causal: query i sees the keys up to i + Sk - Sq.  A query without a key
-    gives a zero row and sends no gradient.  scale: a positive number, default 1 / sqrt(dh).  p_drop: dropout on the
-    probabilities from the library's stream (seed, site)."""
+    gives a zero row and sends no gradient.  What no key_mask takes out has to be finite, also where only the causal order hides it.
+    scale: a positive number, default 1 / sqrt(dh).  p_drop: dropout on the probabilities from the library's stream (seed, site).
+    Deterministic.  Forward and backward can be captured into a graph (a fixed seed replays the same dropout); as with every torch
+    backward, drop what an eager pass over the same leaves left alive (its loss or outputs) before capturing one."""
     q = _seq(q, "q", 4)
     k, v = _seq(k, "k", 4, q), _seq(v, "v", 4, q)
     N, Sq, H, dh = q.shape
@@ -901,7 +905,7 @@ class _LinearAttention(torch.autograd.Function):
         (N, S, H, dk), dv = q.shape, v.shape[3]
         g = torch.zeros(N, S, H, dv, dtype=q.dtype, device=q.device) if g is None else g.contiguous()
         glast = None if glast is None else glast.contiguous()
-        dq, dk_, dv_ = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk_, dv_ = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         dstate = torch.empty(N, H, dk, dv, dtype=torch.float32, device=q.device) if ctx.needs_input_grad[5] else None
         L = lib()
         with _on_device(q):
@@ -941,7 +945,8 @@ def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
     v [N,S,H,dv], fp32 or bf16, any strides with a dense innermost axis, widths up to 128 -> (o [N,S,H,dv], the state after the last
     token [N,H,dk,dv] fp32).  log_decay [H] fp32, <= 0, a constant without gradient.  lens [N]: sequence n has lens[n] tokens (taken
     into [0, S]); o is zero behind them and the state stops there.  state: the state to start from (default zero), as an earlier call
-    or linear_attention_step left it.  scale: default 1 / sqrt(dk).  Differentiable in q, k, v and state."""
+    or linear_attention_step left it.  scale: default 1 / sqrt(dk).  Differentiable in q, k, v and state.  Deterministic; capture as
+    for attention.  Tokens within the length have to be finite."""
     q, k, v, log_decay, state, scale = _linear_args("linear_attention", q, k, v, log_decay, state, scale, 4)
     if lens is not None:
         lens = _same_device(_i64(lens, "lens"), "lens", q.device)
