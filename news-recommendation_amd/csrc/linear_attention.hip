@@ -23,6 +23,11 @@
 // Rounding (bf16): the decayed scores, and the state where a query meets it, are rounded to bf16 as operands of a product (half a
 // step each, against an output of the same type); what goes INTO the state is not (Weighed), and every sum, and the state from chunk
 // to chunk, is fp32.
+//
+// Measured (MI355X, bf16, heads of 64).  What bounds it is the chain through the state: a wave goes through its tiles one after the
+// other, about 7300 cycles per 64 tokens (scores and output 1180 and state 1330 per chunk, stores 400, LDS 510, loads 430), with 2.25
+// waves per SIMD in the backward of 32 x 12 heads and fewer in the forward.  32 sequences up to 1000 tokens, 12 heads: forward 73 us
+// (1.2 TB/s), backward 111 us.  2 x 16384 tokens, 12 heads, in 37 segments: segment sums 26 us, scan 11 us, output 50 us.
 #include "linear_attention.h"
 #include "attention_long_dev.h"
 #include <algorithm>
@@ -360,7 +365,8 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
 }
 
 // ---------------------------------------------------------------- one token
-// a workgroup per head: 16-byte pieces of the state's rows over the threads, the row sums meet through LDS in row-group order
+// a workgroup per head: 16-byte pieces of the state's rows over the threads, the row sums meet through LDS in row-group order.
+// Bound by reading and writing the state: 512 x 12 heads of 64 x 64 in 38 us, 5.3 TB/s (a large copy: 4.9); 12 heads of 25: 4 us.
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void lin_step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                                                        const float* __restrict__ log_decay, const float* state, int H, int dk, int dv, int lanes,
