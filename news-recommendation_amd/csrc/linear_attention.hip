@@ -15,7 +15,7 @@
 // neighbours on one XCD, so that what they read twice comes from its L2.
 //
 // Work split.  A wave owns 32 columns of z / o and of the state, which stays in its registers in fp32 (rows a, column b: a D tile,
-// mma.h) for the whole walk; a workgroup has one wave per 32 columns.  Registers feed both products of the state: as D tiles they
+// mma.h) for the whole walk; a workgroup has one wave per 32 columns (bf16 heads of up to 64: two, lin_pair_kernel).  Registers feed both products of the state: as D tiles they
 // are the A operand of o^T += S^T x^T without a transpose, and the z fragments are the A operand of o^T += z^T A^T and the B
 // operand of S += y^T z.  When heads * sequences do not fill the chip the tokens are also cut into segments: every segment's own
 // sum first (lin_state), a scan over them (lin_scan), then the walk with the right starting states.
@@ -24,10 +24,11 @@
 // step each, against an output of the same type); what goes INTO the state is not (Weighed), and every sum, and the state from chunk
 // to chunk, is fp32.
 //
-// Measured (MI355X, bf16, heads of 64).  What bounds it is the chain through the state: a wave goes through its tiles one after the
-// other, about 7300 cycles per 64 tokens (scores and output 1180 and state 1330 per chunk, stores 400, LDS 510, loads 430), with 2.25
-// waves per SIMD in the backward of 32 x 12 heads and fewer in the forward.  32 sequences up to 1000 tokens, 12 heads: forward 73 us
-// (1.2 TB/s), backward 111 us.  2 x 16384 tokens, 12 heads, in 37 segments: segment sums 26 us, scan 11 us, output 50 us.
+// Measured (MI355X, bf16, heads of 64).  What bounds it is the chain through the state: the tiles of a sequence follow one another, and
+// one wave for everything took about 7300 cycles per 64 tokens (scores and output 1180 and state 1330 per chunk, stores 400, LDS 510,
+// loads 430), which the pairs of waves divide.  32 sequences up to 1000 tokens, 12 heads: forward 60 us (73 with one wave), backward 100
+// (111).  2 x 16384 tokens, 12 heads, in 32 segments: segment sums 26 us, scan 9 us, output 45 us (1.6 TB/s in all, of 2.5 with the
+// second read of k and v).  128 x 1000 tokens, 12 heads: forward 201 us, 3.9 TB/s.
 #include "linear_attention.h"
 #include "attention_long_dev.h"
 #include <algorithm>
@@ -137,8 +138,8 @@ __device__ __forceinline__ float add_weight(float a2, int i, int m, int rev, flo
 }
 
 // the tiles of C tokens that a workgroup walks, the next one on its way from memory while one is worked on
-template <class T, int DA, int DB, bool VEC, bool OUT> struct Walk {
-    static constexpr int NT = 2 * DB, PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, C = TILE<T>;
+template <class T, int DA, int DB, bool VEC, bool OUT, int NT = 2 * DB> struct Walk {
+    static constexpr int PA = DA + Ty<T>::PAD, PB = DB + Ty<T>::PAD, C = TILE<T>;
     static constexpr size_t LDS = ((OUT ? 2 : 1) * PA + PB) * C * sizeof(T) + C * 4 + (OUT ? 64 * 4 : 0);
     typedef Lds<T, C, DA> LA;
     typedef Lds<T, C, DB> LB;
@@ -364,6 +365,125 @@ __global__ __launch_bounds__(2 * DB, (DA * sizeof(T) <= 128 ? 3 : (DA * sizeof(T
     }
 }
 
+// The same for bf16 heads of up to 64: a pair of waves per 32 columns, one that carries the state through the tiles and hands it on, in
+// bf16, as the fragments that the other multiplies while the first goes on.  The chain of a sequence is then the longer of the two
+// halves, not their sum.  A tile's second chunk meets the first one's tokens directly (one more block of scores), so that both waves
+// work on the same tile and one state per tile is handed over.  (One wave for both, 40 x 12 heads of 1000 x 64: forward 66 us, backward
+// 178; pairs 55 and 153.  128 x 12 heads: 223 and 519; 201 and 471.  Wider heads and fp32 would not leave the LDS for it.)
+template <int DA, int DB> constexpr bool PAIRED = DA <= 64 && DB <= 64;
+template <int DA, int DB, bool VEC, bool EXACT>
+__global__ __launch_bounds__(4 * DB, 3) void lin_pair_kernel(const Args a) {
+    typedef __bf16 T;
+    constexpr int NT = 4 * DB, NB = DB / 32, AT = DA / 32, KA = DA / 16;
+    typedef Walk<T, DA, DB, VEC, true, NT> W;
+    static_assert(W::C == 64 && W::LDS % 16 == 0, "two chunks per tile");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool carry = w >= NB;
+    const int wb = carry ? w - NB : w, b = 32 * wb + l31;
+    const Place at(a);
+    const Job& J = a.job[at.job];
+    W walk(at, J, smem);
+    T* op = static_cast<T*>(J.o) + at.n * J.so.n + at.h * J.so.h;
+    const int64_t E = (int64_t)J.da * J.db;
+    typename W::Set set;
+    walk.setup(set, J, tid);
+    walk.fetch(set, 0);
+    // decays between tokens of one chunk, by (row j) - (column i) + 31 (zero on the side that the sum leaves out), and of two chunks
+    float *near = walk.wu + W::C, *far = near + 64;
+    if (tid < 64) {
+        const int d = J.rev ? tid - 31 : 31 - tid;
+        near[tid] = d >= 0 ? J.amul * power(at.a2, d) : 0.f;
+    } else if (tid < 128) {
+        far[tid - 64] = J.amul * power(at.a2, J.rev ? tid - 63 : 127 - tid);
+    }
+    bf16x8* slot = reinterpret_cast<bf16x8*>(smem + W::LDS + 64 * 4) + wb * AT * 2 * 64 + lane;         // [2][NB][AT * 2][64]
+    constexpr int SLOT = NB * AT * 2 * 64;
+    if (carry) {
+        f32x16 S[AT];
+        const float* src = a.G > 1 ? J.seg + (at.nh * a.G + at.seg) * E : (J.init ? J.init + at.nh * E : nullptr);
+        const bool turned = a.G == 1 && J.init_t;
+#pragma unroll
+        for (int x = 0; x < AT; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * x + tile_row(r, h);
+                S[x][r] = src && row < J.da && b < J.db ? src[turned ? b * J.da + row : row * J.db + b] : 0.f;
+            }
+        for (int t = 0; t < walk.nc; ++t) {
+#pragma unroll
+            for (int x = 0; x < 2 * AT; ++x) slot[(t & 1) * SLOT + 64 * x] = tile_frag<T>(S[x >> 1], x & 1);
+            const int m = walk.put(set, t, tid);
+            walk.fetch(set, t + 1);
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                const int it = walk.rev ? 1 - u : u, mi = min(32, m - 32 * it);
+                if (mi <= 0) continue;
+                typename Ty<T>::Frag zf[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) zf[kb] = col_frag<W::PB>(walk.Zs, 32 * it + 16 * kb, 32 * wb, lane);
+                absorb<T, W::PA, AT, (EXACT ? 3 : 2)>(S, walk.Ys, walk.wu, zf, power(at.a2, mi), it, lane);
+            }
+        }
+        if (EXACT && J.last && b < J.db)
+#pragma unroll
+            for (int x = 0; x < AT; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = 32 * x + tile_row(r, h);
+                    if (row < J.da) J.last[at.nh * E + row * J.db + b] = S[x][r];
+                }
+    } else {
+        const int diag = 31 + 4 * h - l31;
+        const float imul = J.imul;
+        const int64_t ostep = J.so.s;
+        const int db = J.db;
+        for (int t = 0; t < walk.nc; ++t) {
+            const int t0 = at.s0 + W::C * walk.tile(t), m = walk.put(set, t, tid);
+            walk.fetch(set, t + 1);
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                const int it = walk.rev ? 1 - u : u, mi = min(32, m - 32 * it);
+                if (mi <= 0) continue;
+                const T* xr = walk.Xs + (32 * it + l31) * W::PA;
+                f32x16 o = zero16();
+#pragma unroll
+                for (int y = 0; y < AT; ++y)
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) o = mul(slot[(t & 1) * SLOT + 64 * (2 * y + k2)], spread_frag(xr + 32 * y + 16 * k2 + 4 * h), o);
+                const float wi = imul * power(at.a2, walk.rev ? max(m - 1 - 32 * it - l31, 0) : 32 * it + l31 + 1);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[r] *= wi;
+                auto meet = [&](int jt, const float* decay) {                    // the tokens of half jt
+                    const T* yr = walk.Ys + (32 * jt + l31) * W::PA;
+                    f32x16 x = zero16();
+#pragma unroll
+                    for (int k = 0; k < KA; ++k) x = mul(near_frag(yr + 16 * k + 8 * h), near_frag(xr + 16 * k + 8 * h), x);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] *= decay[tile_row(r, 0)];
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) o = mul(col_frag<W::PB>(walk.Zs, 32 * jt + 16 * kb, 32 * wb, lane), tile_frag<T>(x, kb), o);
+                };
+                meet(it, near + diag);
+                if (u && m > 32) meet(1 - it, far + diag);
+                if (l31 < mi) {
+                    T* row = op + (t0 + 32 * it + l31) * ostep;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int col = 32 * wb + 8 * q + 4 * h;
+                        store4<VEC>(row + col, f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]}, db - col);
+                    }
+                }
+            }
+        }
+    }
+    // rows behind the sequence's length
+    for (int x = tid; x < (at.send - at.s1) * J.db; x += NT) {
+        const int row = x / J.db;
+        op[(int64_t)(at.s1 + row) * J.so.s + (x - row * J.db)] = (T)0.f;
+    }
+}
+
 // ---------------------------------------------------------------- one token
 // a workgroup per head: 16-byte pieces of the state's rows over the threads, the row sums meet through LDS in row-group order.
 // Bound by reading and writing the state: 512 x 12 heads of 64 x 64 in 38 us, 5.3 TB/s (a large copy: 4.9); 12 heads of 25: 4 us.
@@ -410,13 +530,15 @@ __global__ __launch_bounds__(256) void lin_step_kernel(const T* __restrict__ q, 
 }
 
 // ---------------------------------------------------------------- host
-// heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each, at least three of them: the extra
-// pass reads y and z again (32 x 12 heads of 1000 x 64: 76 us whole, 81 us in two; 2 x 12 of 16384: 88 us in 37)
-static void cut(Args& a) {
-    const int64_t blocks = a.jobs * a.N * a.H;
+// heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each, at least three of them, and only past
+// 1024 tokens: the extra pass reads y and z again, and a scan follows it (16 x 12 ragged heads of 1000 x 64: 35 us whole, 46 us in
+// three; 2 x 12 of 16384: 69 us in 32).  Aimed at as many workgroups as the chip holds at once: three per CU of the pair kernel (512:
+// 73 us, 1024: 83), four of the other.
+static void cut(Args& a, bool bf16) {
+    const int64_t blocks = a.jobs * a.N * a.H, aim = bf16 && a.job[0].da <= 64 && a.job[0].db <= 64 ? 768 : 1024;
     a.G = 1; a.per = (a.S + UNIT - 1) / UNIT * UNIT;
-    const int64_t want = std::min<int64_t>(blocks > 0 ? 1024 / blocks : 0, a.S / 256);
-    if (want < 3) return;
+    const int64_t want = std::min<int64_t>(blocks > 0 ? aim / blocks : 0, a.S / 256);
+    if (want < 3 || a.S <= 1024) return;
     a.per = (int)((((int64_t)a.S + want - 1) / want + UNIT - 1) / UNIT * UNIT);
     a.G = (a.S + a.per - 1) / a.per;
 }
@@ -438,12 +560,17 @@ template <class T, int DA, int DB, bool VEC> static int launch(const Args& a, hi
     }
     bool exact = false;
     for (int j = 0; j < a.jobs; ++j) exact = exact || (a.job[j].last && a.G == 1);
-    auto go = [&](auto kernel) {
-        if (out_lds > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)out_lds);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(2 * DB), out_lds, s, a);
+    auto go = [&](auto kernel, int threads, size_t lds) {
+        if (lds > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
         return check_launch("linear_attention");
     };
-    return exact ? go(&lin_out_kernel<T, DA, DB, VEC, true>) : go(&lin_out_kernel<T, DA, DB, VEC, false>);
+    if constexpr (sizeof(T) == 2 && PAIRED<DA, DB>) {
+        constexpr size_t lds = Walk<T, DA, DB, VEC, true, 4 * DB>::LDS + 64 * 4 + (size_t)2 * DA * DB * 2;
+        return exact ? go(&lin_pair_kernel<DA, DB, VEC, true>, 4 * DB, lds) : go(&lin_pair_kernel<DA, DB, VEC, false>, 4 * DB, lds);
+    } else {
+        return exact ? go(&lin_out_kernel<T, DA, DB, VEC, true>, 2 * DB, out_lds) : go(&lin_out_kernel<T, DA, DB, VEC, false>, 2 * DB, out_lds);
+    }
 }
 template <class T, int DA, bool VEC> static int pick_b(const Args& a, hipStream_t s) {
     const int b = pad32(a.job[0].db);
@@ -483,7 +610,7 @@ static Args fwd_args(const LinProblem& p, void* out, float* last) {
     Args a = base(p);
     a.jobs = 1;
     a.job[0] = Job{p.q, p.k, p.v, p.sq, p.sk, p.sv, dense(p.S, p.H, p.dv), out, p.state, 0, last, nullptr, p.dk, p.dv, 0, p.scale, p.scale, 1.f};
-    cut(a);
+    cut(a, p.bf16);
     return a;
 }
 // the three products of the backward: one launch, or two where dk and dv are padded to different widths
@@ -496,12 +623,12 @@ static int bwd_args(const LinProblem& p, const void* g, const float* dlast, void
     a[0].job[0] = jq; a[0].job[1] = jk; a[0].jobs = 2;
     if (pad32(p.dk) == pad32(p.dv)) {
         a[0].job[2] = jv; a[0].jobs = 3;
-        cut(a[0]);
+        cut(a[0], p.bf16);
         return 1;
     }
     a[1].job[0] = jv; a[1].jobs = 1;
-    cut(a[0]);
-    cut(a[1]);
+    cut(a[0], p.bf16);
+    cut(a[1], p.bf16);
     return 2;
 }
 
