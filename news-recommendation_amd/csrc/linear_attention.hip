@@ -27,8 +27,8 @@
 // Measured (MI355X, bf16, heads of 64).  What bounds it is the chain through the state: the tiles of a sequence follow one another, and
 // one wave for everything took about 7300 cycles per 64 tokens (scores and output 1180 and state 1330 per chunk, stores 400, LDS 510,
 // loads 430), which the pairs of waves divide.  32 sequences up to 1000 tokens, 12 heads: forward 60 us (73 with one wave), backward 100
-// (111).  2 x 16384 tokens, 12 heads, in 32 segments: segment sums 26 us, scan 9 us, output 45 us (1.6 TB/s in all, of 2.5 with the
-// second read of k and v).  128 x 1000 tokens, 12 heads: forward 201 us, 3.9 TB/s.
+// (111).  2 x 16384 tokens, 12 heads, in 32 segments: segment sums 26 us, scan 9 us, output 45 us: 2.5 TB/s in all, 3.8 with the
+// second read of k and v.  128 x 1000 tokens, 12 heads: forward 201 us, 3.9 TB/s.
 #include "linear_attention.h"
 #include "attention_long_dev.h"
 #include <algorithm>

@@ -236,6 +236,22 @@ def test_captured_and_replayed(ops, size):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("name", [0, 1, 2], ids=["q", "k", "v"])
+@pytest.mark.parametrize("size", [(2, 75, 75, 2, 2, 64), (2, 3, 1100, 4, 2, 32)], ids=lambda s: "x".join(map(str, s)))
+def test_one_row_for_all_positions(ops, size, name, dtype):
+    """an operand broadcast along the positions (stride 0), tiles that end inside a sequence: the same bits as its copy"""
+    ts = list(make(19, *size, dtype))
+    m = make_mask("prefix", 2, size[0], size[2])
+    spread = ts[name][:, :1].expand(ts[name].shape)
+    got = []
+    for x in (spread, spread.contiguous()):
+        ts[name] = x
+        got.append(run(ops, *ts, key_mask=m, causal=size[1] == size[2]))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_two_graphs_do_not_share_scratch(ops):
     a, b = make(1, 1, 3, 3000, 4, 2, 64, BF16), make(2, 1, 3, 3000, 4, 2, 64, BF16)
     with torch.no_grad():

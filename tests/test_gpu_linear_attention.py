@@ -213,6 +213,28 @@ def test_strided_views(ops, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("S", [75, 1300])
+def test_one_row_for_all_tokens(ops, S, name, dtype):
+    """an operand broadcast along the tokens (stride 0), sequences that end inside a tile: the same bits as its copy"""
+    N, H, d = 3, 2, 64
+    t, a = make(17, N, S, H, d, d, dtype), decays(H)
+    lens = torch.tensor([S, S - 9, 33], device="cuda")
+    row = t[name][:, :1]
+
+    def both(x):
+        ops_in = {n: t[n].detach() for n in ("q", "k", "v")}
+        ops_in[name] = x
+        leaves = [ops_in[n].requires_grad_(True) for n in ("q", "k", "v")]
+        o, last = ops.linear_attention(*leaves, a, lens)
+        return (o, last) + torch.autograd.grad((o, last), leaves, (t["do"], torch.ones_like(last)))
+
+    spread = row.detach().expand(N, S, H, d)
+    for x, y in zip(both(spread), both(spread.contiguous())):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("N,H,dk,dv", [(1, 1, 1, 1), (3, 2, 5, 7), (2, 12, 25, 25), (5, 3, 64, 64), (2, 2, 128, 128), (3, 1, 16, 128), (2, 4, 100, 36)])
 def test_step(ops, N, H, dk, dv, dtype):
     """one token.  Bound: the new state is one fused product and sum of fp32 operands and a decay known to 2^-22; the output a dot of
