@@ -959,12 +959,14 @@ def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None):
     """one token of linear_attention for every sequence: q / k [N,H,dk], v [N,H,dv], state [N,H,dk,dv] fp32 -> o [N,H,dv].  The new
-    state goes to out_state (dense, may be state itself), by default over state.  Inference only (no autograd)."""
+    state goes to out_state (dense, may be state itself), by default over state.  Inference only: refused where a gradient would be expected."""
     if state is None:
         raise NewsrecError("linear_attention_step: needs a state")
     given = state
     q, k, v, log_decay, state, scale = _linear_args("linear_attention_step", q, k, v, log_decay, state, scale, 3)
     out_state = given if out_state is None else out_state
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise NewsrecError("linear_attention_step: has no gradient (call it under torch.no_grad, or linear_attention for one token)")
     if (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != q.device or out_state.shape != state.shape
             or not out_state.is_contiguous()):
         raise NewsrecError("linear_attention_step: the state to write must be a dense fp32 tensor of the state's shape on the same device")

@@ -380,3 +380,18 @@ def test_refusals(ops):
     ops.linear_attention_step(t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], a, held)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+def test_step_where_a_gradient_would_be_expected(ops):
+    t = make(18, 2, 1, 2, 16, 16, F32)
+    q, k, v = (t[n][:, 0] for n in ("q", "k", "v"))
+    a, state = decays(2), torch.zeros(2, 2, 16, 16, device="cuda")
+    want = ops.linear_attention_step(q, k, v, a, state.clone())
+    args = [q, k, v, state]
+    for i in range(4):
+        leaf = [x.clone().requires_grad_(i == j) for j, x in enumerate(args)]
+        with pytest.raises(Exception, match="no gradient"):
+            ops.linear_attention_step(*leaf[:3], a, leaf[3])
+        assert not bool(leaf[3].any())
+        with torch.no_grad():
+            assert torch.equal(ops.linear_attention_step(*leaf[:3], a, leaf[3].detach()), want)
