@@ -112,7 +112,9 @@ __global__ __launch_bounds__(256, (DkvCfg<T, DHP>::WAVES)) void attn_dkv_kernel(
         sq.load(static_cast<const T*>(a.q) + n * a.sq.n + i0 * a.sq.s + head * a.sq.h, rows);
         sg.load(static_cast<const T*>(a.dout) + n * a.sdo.n + i0 * a.sdo.s + head * a.sdo.h, rows);
         if (tid < QT) {
-            st[0] = 0.f; st[1] = INFINITY; st[2] = 0.f;                          // (no row: its probabilities come out as zero)
+            // no row: exp(-INFINITY) whatever its scores are.  (They are not always 0: where rows share memory a tile holds more of it
+            // behind the last one, and exp(score - 0) * (1 / INFINITY) was inf * 0 for fp32 scores past 88.)
+            st[0] = st[1] = INFINITY; st[2] = 0.f;
             if (tid < rows) {
                 const int64_t x = (n * a.H + head) * a.Sq + i0 + tid;
                 st[0] = a.row_max[x];

@@ -84,8 +84,9 @@ __device__ __forceinline__ uint32_t keep4(const Args& a, uint64_t idx) {
 }
 
 // Rows [0, rows) of a [ROWS x DHP] tile on their way from global memory into LDS, 16 bytes per piece: `load` only issues the loads,
-// `store` waits.  Rows past `rows` and columns past dh read as zero.  VEC: buffer loads whose bounds check does that, with one
-// 32-bit offset per thread (the host checks that a tile's offsets fit); otherwise element by element.
+// `store` waits.  Rows past `rows` and columns past dh read as zero, except that rows which share memory (a row stride below dh) may
+// go on with what is left of it: finite where the rows are, and no memory of others.  VEC: buffer loads whose bounds check does that,
+// with one 32-bit offset per thread (the host checks that a tile's offsets fit); otherwise element by element.
 template <class T, int DHP, int ROWS, bool VEC, int NT = 256>
 struct Stage {
     static constexpr int E = Ty<T>::E, PER_ROW = DHP / E, NCH = ROWS * PER_ROW / NT, STEP = NT / PER_ROW;
