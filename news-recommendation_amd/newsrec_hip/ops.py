@@ -12,6 +12,7 @@ import os
 import time
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -488,6 +489,15 @@ def _same_device(t, name, device):
     return t
 
 
+def _no_tangent(what, *tensors):
+    """a dual tensor of forward-mode differentiation does not require a gradient, so the call would go past autograd and lose its tangent
+    without a word.  (Outside of forward mode nothing is asked of the tensors.)"""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NewsrecError(f"{what}: has no forward-mode derivative")
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -566,7 +576,9 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
     gives a zero row and sends no gradient.  What no key_mask takes out has to be finite, also where only the causal order hides it.
     scale: a positive number, default 1 / sqrt(dh).  p_drop: dropout on the probabilities from the library's stream (seed, site).
     Deterministic.  Forward and backward can be captured into a graph (a fixed seed replays the same dropout); as with every torch
-    backward, drop what an eager pass over the same leaves left alive (its loss or outputs) before capturing one."""
+    backward, drop what an eager pass over the same leaves left alive (its loss or outputs) before capturing one.  Forward-mode
+    differentiation is refused."""
+    _no_tangent("attention", q, k, v)
     q = _seq(q, "q", 4)
     k, v = _seq(k, "k", 4, q), _seq(v, "v", 4, q)
     N, Sq, H, dh = q.shape
@@ -946,7 +958,8 @@ def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
     token [N,H,dk,dv] fp32).  log_decay [H] fp32, <= 0, a constant without gradient.  lens [N]: sequence n has lens[n] tokens (taken
     into [0, S]); o is zero behind them and the state stops there.  state: the state to start from (default zero), as an earlier call
     or linear_attention_step left it.  scale: default 1 / sqrt(dk).  Differentiable in q, k, v and state.  Deterministic; capture as
-    for attention.  Tokens within the length have to be finite."""
+    for attention.  Tokens within the length have to be finite.  Forward-mode differentiation is refused."""
+    _no_tangent("linear_attention", q, k, v, log_decay, state)
     q, k, v, log_decay, state, scale = _linear_args("linear_attention", q, k, v, log_decay, state, scale, 4)
     if lens is not None:
         lens = _same_device(_i64(lens, "lens"), "lens", q.device)
@@ -962,6 +975,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None)
     state goes to out_state (dense, may be state itself), by default over state.  Inference only: refused where a gradient would be expected."""
     if state is None:
         raise NewsrecError("linear_attention_step: needs a state")
+    _no_tangent("linear_attention_step", q, k, v, log_decay, state, out_state)
     given = state
     q, k, v, log_decay, state, scale = _linear_args("linear_attention_step", q, k, v, log_decay, state, scale, 3)
     out_state = given if out_state is None else out_state

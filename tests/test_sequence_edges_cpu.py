@@ -1,0 +1,30 @@
+"""what ops.attention, ops.linear_attention and ops.linear_attention_step refuse before any device call"""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from newsrec_hip import ops
+from newsrec_hip._lib import NewsrecError
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "log_decay", "state", "out_state"])
+def test_forward_mode_is_refused(name):
+    """a dual tensor has requires_grad == False: a call that looks at no more than that would hand back an output without a tangent"""
+    r = lambda *s: torch.ones(*s)                                                          # noqa: E731
+    whole = dict(q=r(1, 3, 2, 4), k=r(1, 3, 2, 4), v=r(1, 3, 2, 4))
+    rec = dict(whole, log_decay=r(2), state=r(1, 2, 4, 4))
+    step = dict({n: t[:, 0] for n, t in whole.items()}, log_decay=r(2), state=r(1, 2, 4, 4), out_state=r(1, 2, 4, 4))
+    for op, args in ((ops.attention, whole), (ops.linear_attention, rec), (ops.linear_attention_step, step)):
+        if name not in args:
+            continue
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+            with pytest.raises(NewsrecError, match="forward-mode"):
+                op(**{**args, name: dual})
+            with torch.no_grad(), pytest.raises(NewsrecError, match="forward-mode"):
+                op(**{**args, name: dual})
+        with pytest.raises(NewsrecError, match="forward-mode"):
+            torch.func.jvp(lambda t: op(**{**args, name: t}), (args[name],), (torch.ones_like(args[name]),))
+        with pytest.raises(NewsrecError, match="ROCm"):           # outside, the next check speaks
+            op(**args)
