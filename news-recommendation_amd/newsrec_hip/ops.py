@@ -972,10 +972,13 @@ def linear_attention(q, k, v, log_decay, lens=None, state=None, scale=None):
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None, out_state=None):
     """one token of linear_attention for every sequence: q / k [N,H,dk], v [N,H,dv], state [N,H,dk,dv] fp32 -> o [N,H,dv].  The new
-    state goes to out_state (dense, may be state itself), by default over state.  Inference only: refused where a gradient would be expected."""
+    state goes to out_state (dense, may be state itself), by default over state.  Inference only: refused where a gradient would be expected,
+    of the inputs or of what out_state held."""
     if state is None:
         raise NewsrecError("linear_attention_step: needs a state")
     _no_tangent("linear_attention_step", q, k, v, log_decay, state, out_state)
+    if torch.is_grad_enabled() and isinstance(out_state, torch.Tensor) and out_state.requires_grad:
+        raise NewsrecError("linear_attention_step: out_state belongs to a graph that expects its gradient (give a tensor of its own, or call under torch.no_grad)")
     given = state
     q, k, v, log_decay, state, scale = _linear_args("linear_attention_step", q, k, v, log_decay, state, scale, 3)
     out_state = given if out_state is None else out_state

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import test_gpu_attention as A
+import test_gpu_linear_attention as L
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -40,3 +41,15 @@ def test_shared_rows_under_large_scores(ops, Sq, step, name, causal, dtype):
     for n, a, b in zip(("o", "dq", "dk", "dv"), *got):
         assert bool(torch.isfinite(b.float()).all()), n
         assert torch.equal(a, b), n
+
+
+def test_a_state_that_belongs_to_a_graph_is_not_written(ops):
+    t, a = L.make(49, 2, 40, 2, 16, 24, F32), L.decays(2)
+    q = t["q"].detach().requires_grad_(True)
+    _, last = ops.linear_attention(q, t["k"], t["v"], a, state=t["state"].clone().requires_grad_(True))
+    held = last.detach().clone()
+    for out in (last, t["state"].clone().requires_grad_(True)):
+        before = out.detach().clone()
+        with pytest.raises(ops.NewsrecError, match="out_state.*gradient"):
+            ops.linear_attention_step(t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], a, held, out_state=out)
+        assert torch.equal(out.detach(), before)

@@ -28,3 +28,15 @@ def test_forward_mode_is_refused(name):
             torch.func.jvp(lambda t: op(**{**args, name: t}), (args[name],), (torch.ones_like(args[name]),))
         with pytest.raises(NewsrecError, match="ROCm"):           # outside, the next check speaks
             op(**args)
+
+
+def test_a_state_that_belongs_to_a_graph_is_not_written():
+    """torch refuses a tensor that requires a gradient as an out= argument; so does the step, leaf or not"""
+    r = lambda *s: torch.ones(*s)                                                          # noqa: E731
+    args = dict(q=r(1, 2, 4), k=r(1, 2, 4), v=r(1, 2, 4), log_decay=r(2), state=r(1, 2, 4, 4))
+    leaf = r(1, 2, 4, 4).requires_grad_(True)
+    for held in (leaf, leaf * 2):
+        with pytest.raises(NewsrecError, match="out_state.*gradient"):
+            ops.linear_attention_step(**args, out_state=held)
+        with torch.no_grad(), pytest.raises(NewsrecError, match="ROCm"):                   # as for out=, no_grad allows it
+            ops.linear_attention_step(**args, out_state=held)
