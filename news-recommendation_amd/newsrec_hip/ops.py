@@ -498,6 +498,16 @@ def _no_tangent(what, *tensors):
                 raise NewsrecError(f"{what}: has no forward-mode derivative")
 
 
+def _scale(what, scale):
+    """a factor that crosses the C boundary in fp32"""
+    scale = float(scale)
+    if not abs(scale) <= _FP32_MAX:
+        raise NewsrecError(f"{what}: scale {scale} is not a number within fp32's range")
+    return scale
+
+
+_FP32_MIN = 2.0 ** -149
+_FP32_MAX = (2.0 - 2.0 ** -23) * 2.0 ** 127
 _HERE = contextlib.nullcontext()
 
 
@@ -579,6 +589,10 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
     backward, drop what an eager pass over the same leaves left alive (its loss or outputs) before capturing one.  Forward-mode
     differentiation is refused."""
     _no_tangent("attention", q, k, v)
+    if scale is not None:
+        scale = _scale("attention", scale)
+        if not scale >= _FP32_MIN:
+            raise NewsrecError(f"attention: scale {scale} is not a positive number of fp32")
     q = _seq(q, "q", 4)
     k, v = _seq(k, "k", 4, q), _seq(v, "v", 4, q)
     N, Sq, H, dh = q.shape
@@ -592,9 +606,7 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None, p_drop=0.0, seed
         key_mask = _same_device(_i64(key_mask, "key_mask"), "key_mask", q.device)
         if tuple(key_mask.shape) != (N, k.shape[1]):
             raise NewsrecError(f"attention: key_mask {tuple(key_mask.shape)} for {N} sequences of {k.shape[1]} keys")
-    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise NewsrecError(f"attention: scale {scale} is not a positive number")
+    scale = 1.0 / math.sqrt(dh) if scale is None else scale
     if not 0.0 <= p_drop < 1.0:
         raise NewsrecError(f"attention: p_drop {p_drop} not in [0, 1)")
     cfg = (1 if causal else 0, scale, float(p_drop), int(seed) & 0xFFFFFFFFFFFFFFFF, int(site) & 0xFFFFFFFF)
@@ -930,6 +942,7 @@ class _LinearAttention(torch.autograd.Function):
 
 
 def _linear_args(what, q, k, v, log_decay, state, scale, dims):
+    scale = None if scale is None else _scale(what, scale)
     q = _seq(q, "q", dims)
     k, v = _seq(k, "k", dims, q), _seq(v, "v", dims, q)
     if k.shape != q.shape or v.shape[:-1] != q.shape[:-1]:
@@ -946,9 +959,7 @@ def _linear_args(what, q, k, v, log_decay, state, scale, dims):
         state = _same_device(_f32(state, "state"), "state", q.device)
         if tuple(state.shape) != (N, H, dk, dv):
             raise NewsrecError(f"{what}: state {tuple(state.shape)}, expected {(N, H, dk, dv)}")
-    scale = 1.0 / math.sqrt(dk) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise NewsrecError(f"{what}: scale {scale} is not a number")
+    scale = 1.0 / math.sqrt(dk) if scale is None else scale
     return q, k, v, log_decay, state, scale
 
 

@@ -1,4 +1,5 @@
 """what ops.attention, ops.linear_attention and ops.linear_attention_step refuse before any device call"""
+import math
 
 import pytest
 import torch
@@ -40,3 +41,16 @@ def test_a_state_that_belongs_to_a_graph_is_not_written():
             ops.linear_attention_step(**args, out_state=held)
         with torch.no_grad(), pytest.raises(NewsrecError, match="ROCm"):                   # as for out=, no_grad allows it
             ops.linear_attention_step(**args, out_state=held)
+
+
+@pytest.mark.parametrize("scale", [1e39, 3.5e38, 1e300, math.inf, math.nan])
+def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
+    x, one = torch.ones(1, 3, 2, 4), torch.ones(1, 2, 4)
+    for s in (scale, -scale):
+        for call in (lambda: ops.attention(x, x, x, scale=s), lambda: ops.linear_attention(x, x, x, torch.zeros(2), scale=s),
+                     lambda: ops.linear_attention_step(one, one, one, torch.zeros(2), torch.zeros(1, 2, 4, 4), scale=s)):
+            with pytest.raises(NewsrecError, match="scale"):
+                call()
+    for s in (0.0, -1.0, 1e-46):                             # (1e-46 is zero in fp32)
+        with pytest.raises(NewsrecError, match="scale"):
+            ops.attention(x, x, x, scale=s)
