@@ -142,7 +142,7 @@ int nr_add_layernorm_bwd_noalloc_f32(const float* dy, const float* s, const floa
  * mask_mode 0: masked keys get an additive -1e5 in fp32 before the softmax (attention.py:44-49,90);
  * mask_mode 1: masked keys are excluded and a sequence without any valid key gets zero probabilities — what
  *   HF BertModel computes under torch SDPA for AllBertNewsEncoder (encoder.py:74; transformers 5.15 / torch 2.10).
- * Any S; head dims up to 128.  Sequences of S <= 128 run on kernels that hold a whole head at once, longer ones (and the head dims
+ * Any S (up to 2^30); head dims up to 128.  Sequences of S <= 128 run on kernels that hold a whole head at once, longer ones (and the head dims
  * those kernels do not take) on the key-tiled kernels of nr_attention_fwd / _bwd below, which S has no bound for. */
 int nr_mhsa_fwd_f32(const float* qkv, const int64_t* mask, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* ctx, float* row_max, float* row_sum, void* stream);
 int nr_mhsa_bwd_f32(const float* qkv, const int64_t* mask, const float* ctx, const float* dctx, const float* row_max, const float* row_sum, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* dqkv, void* stream);
@@ -163,7 +163,8 @@ int nr_mhsa_bwd_bf16(const void* qkv, const int64_t* mask, const void* dctx, con
  * bf16 numbers each, to fp32 accuracy).  bf16: scores scale * q.k beyond 2^16 cost the gradients accuracy (the row's maximum, in
  * fp32, is off by half a step), beyond 2^30 the output as well.
  * q [N,Sq,H,dh], k / v [N,Sk,G,dh]: dtype 0 = fp32, 1 = bf16; innermost axis dense, the other strides in elements, any (0 as
- * well); multiples of 16 bytes throughout run faster.  out, dout, dq, dk, dv: dense, same dtype.  dh <= 128.
+ * well); multiples of 16 bytes throughout run faster.  out, dout, dq, dk, dv: dense, same dtype.  dh <= 128;
+ * Sk and H / G * Sq up to 2^30, N * G up to 2^31.
  * row_max / row_sum [N,H,Sq] fp32 (NULL in evaluation): the softmax statistics that the backward reuses (for bf16 the maximum is in
  * units of log 2, and may lag behind the true one).
  * Dropout on the probabilities: element index ((n*H + h)*Sq + i)*Sk + j of (seed, site).
@@ -188,7 +189,8 @@ int nr_attention_bwd(const nr_attention* p, const void* out, const void* dout, c
  * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  out_t = scale * q_t S_t  for the tokens t < lens[n] of every sequence (lens [N] int64,
  * taken into [0, S]; NULL: all S): a recurrent user tower beside nr_gru_fwd_f32 (RnnUserEncoder, encoder.py:204-233) whose tokens
  * do not wait for each other.  out rows behind a sequence's length are zero; what q / k / v hold there is never used.
- * q / k [N,S,H,dk], v [N,S,H,dv]: dtype 0 = fp32, 1 = bf16, innermost axis dense, other strides in elements; dk, dv <= 128.
+ * q / k [N,S,H,dk], v [N,S,H,dv]: dtype 0 = fp32, 1 = bf16, innermost axis dense, other strides in elements; dk, dv <= 128,
+ * S < 2^30, N * H up to 2^31.
  * log_decay [H] fp32, <= 0 (-INFINITY: no memory) and, like lens, not differentiated.  state / last [N,H,dk,dv] fp32, dense: the
  * state before the first and after the last token (state NULL: zero; last must be given).  out [N,S,H,dv] dense.
  * bwd: dout like out; dlast the gradient of last (NULL: zero); dq / dk / dv dense; dstate the gradient of state (NULL: not wanted).

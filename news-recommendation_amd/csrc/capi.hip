@@ -442,8 +442,14 @@ int nr_add_layernorm_bwd_noalloc_f32(const float* dy, const float* s_in, const f
     return layernorm_bwd(dy, s_in, mean, rstd, gamma, R, (int)D, DC(p_drop, seed, site), ds, dh, dgamma, dbeta, ws, S(stream));
 }
 
+// what goes on in 32-bit integers; the rows of a key-tiled problem count 2^30 at most
+static int mhsa_sizes(const char* what, int64_t Sq, int64_t H, int64_t dh) {
+    NR_UNSUPPORTED(Sq > 0x3fffffff || H > 0x7fffffff || dh > 128, "%s: %lld positions (2^30 at most), %lld heads (2^31) or head dim %lld (128)", what, (long long)Sq, (long long)H, (long long)dh);
+    return NR_OK;
+}
 int nr_mhsa_fwd_f32(const float* qkv, const int64_t* mask, int64_t N, int64_t Sq, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* ctx, float* row_max, float* row_sum, void* stream) {
     NR_CHECK_ARG(N >= 0 && Sq > 0 && H > 0 && dh > 0, "mhsa_fwd: bad sizes");
+    if (int rc = mhsa_sizes("mhsa_fwd", Sq, H, dh)) return rc;
     NR_CHECK_ARG(N == 0 || (qkv && mask && ctx), "mhsa_fwd: null pointer");
     NR_CHECK_ARG((row_max == nullptr) == (row_sum == nullptr), "mhsa_fwd: row_max/row_sum must both be given or both NULL");
     return mhsa_fwd(qkv, mask, ctx, row_max, row_sum, N, (int)Sq, (int)H, (int)dh, DCA(p_drop, seed, site, mask_mode), S(stream));
@@ -451,6 +457,7 @@ int nr_mhsa_fwd_f32(const float* qkv, const int64_t* mask, int64_t N, int64_t Sq
 
 int nr_mhsa_bwd_f32(const float* qkv, const int64_t* mask, const float* ctx, const float* dctx, const float* row_max, const float* row_sum, int64_t N, int64_t Sq, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* dqkv, void* stream) {
     NR_CHECK_ARG(N >= 0 && Sq > 0 && H > 0 && dh > 0, "mhsa_bwd: bad sizes");
+    if (int rc = mhsa_sizes("mhsa_bwd", Sq, H, dh)) return rc;
     NR_CHECK_ARG(N == 0 || (qkv && mask && ctx && dctx && row_max && row_sum && dqkv), "mhsa_bwd: null pointer");
     return mhsa_bwd(qkv, mask, ctx, dctx, row_max, row_sum, dqkv, N, (int)Sq, (int)H, (int)dh, DCA(p_drop, seed, site, mask_mode), S(stream));
 }
@@ -478,7 +485,9 @@ static int attn_problem(const nr_attention* p, AttnProblem* a, const char* what)
     NR_CHECK_ARG(p->p_drop >= 0.f && p->p_drop < 1.f, "%s: p_drop %f not in [0,1)", what, p->p_drop);
     NR_CHECK_ARG(p->scale > 0.f && p->scale < INFINITY, "%s: scale %f is not a positive number", what, p->scale);
     NR_UNSUPPORTED(p->dh > 128, "%s: head dim %lld > 128", what, (long long)p->dh);
-    NR_UNSUPPORTED(p->Sk > 0x3fffffff || p->H / p->G * p->Sq > 0x3fffffff, "%s: %lld keys or %lld rows per key head exceed 2^30", what, (long long)p->Sk, (long long)(p->H / p->G * p->Sq));
+    NR_UNSUPPORTED(p->Sk > 0x3fffffff || p->Sq > 0x3fffffff || p->H > 0x7fffffff || p->H / p->G * p->Sq > 0x3fffffff,
+                   "%s: %lld keys (2^30 at most), %lld heads (2^31) or %lld queries of %lld heads per key head (2^30 rows)", what, (long long)p->Sk, (long long)p->H, (long long)p->Sq, (long long)(p->H / p->G));
+    NR_UNSUPPORTED(p->N > 0x7fffffff / p->G, "%s: %lld sequences of %lld key heads exceed 2^31", what, (long long)p->N, (long long)p->G);
     if (p->N == 0 || p->Sq == 0) return NR_OK;
     NR_CHECK_ARG(p->q && (p->Sk == 0 || (p->k && p->v)), "%s: null pointer", what);
     a->q = p->q; a->k = p->k; a->v = p->v; a->key_mask = p->key_mask;
@@ -535,6 +544,7 @@ static int lin_sizes(const char* what, int64_t N, int64_t S, int64_t H, int64_t 
     NR_CHECK_ARG(fabsf(scale) < INFINITY, "%s: scale %f is not a number", what, scale);
     NR_UNSUPPORTED(dk > 128 || dv > 128, "%s: head dims %lld, %lld > 128", what, (long long)dk, (long long)dv);
     NR_UNSUPPORTED(S > 0x3fffffff || H > 0xffff, "%s: %lld tokens or %lld heads", what, (long long)S, (long long)H);
+    NR_UNSUPPORTED(N > 0x7fffffff / H, "%s: %lld sequences of %lld heads exceed 2^31", what, (long long)N, (long long)H);
     return NR_OK;
 }
 static int lin_problem(const nr_linear_attention* p, LinProblem* a, const char* what) {

@@ -1,5 +1,8 @@
 """what ops.attention, ops.linear_attention and ops.linear_attention_step refuse before any device call"""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -54,3 +57,29 @@ def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
     for s in (0.0, -1.0, 1e-46):                             # (1e-46 is zero in fp32)
         with pytest.raises(NewsrecError, match="scale"):
             ops.attention(x, x, x, scale=s)
+
+
+# sizes whose products or fp32-sized integers wrap: each in a process of its own, since what this refuses used to end it
+HUGE = [("attention", dict(H=1 << 32, G=1 << 32, Sq=1)), ("attention", dict(H=1 << 62, G=1, Sq=8)), ("attention", dict(N=1 << 62, H=4, G=4)),
+        ("attention", dict(N=1 << 40, H=1 << 24, G=1 << 24, Sq=1)), ("linear_attention", dict(N=1 << 62)), ("linear_attention", dict(N=1 << 31, H=4)),
+        ("step", dict(N=1 << 62, H=4)), ("mhsa", dict(S=(1 << 32) + 5)), ("mhsa", dict(S=1 << 30)), ("mhsa", dict(H=1 << 32)), ("mhsa", dict(dh=(1 << 32) + 8))]
+
+
+@pytest.mark.parametrize("what,kw", HUGE, ids=lambda x: x if isinstance(x, str) else "-".join(f"{n}{v}" for n, v in x.items()))
+def test_sizes_past_the_kernels_integers_are_refused(what, kw):
+    calls = {
+        "attention": "L.nr_attention_fwd(d, 16, None, None, None, 0, None), L.nr_attention_bwd(d, 16, 16, 16, 16, 16, 16, 16, 16, None, 0, None), "
+                     "2 * (L.nr_attention_fwd_ws_bytes(d) == 0), 2 * (L.nr_attention_bwd_ws_bytes(d) == 0)",
+        "linear_attention": "L.nr_linear_attention_fwd(d, 16, 16, None, 0, None), L.nr_linear_attention_bwd(d, 16, None, 16, 16, 16, None, None, 0, None), "
+                            "2 * (L.nr_linear_attention_fwd_ws_bytes(d) == 0), 2 * (L.nr_linear_attention_bwd_ws_bytes(d) == 0)",
+        "step": "(L.nr_linear_attention_step(16, 16, 16, 16, 16, d['N'], d['H'], 16, 16, 0, 1.0, 16, 16, None),)",
+        "mhsa": "L.nr_mhsa_fwd_f32(16, 16, 1, d['S'], d['H'], d['dh'], 0.0, 0, 0, 0, 16, 16, 16, None), "
+                "L.nr_mhsa_bwd_f32(16, 16, 16, 16, 16, 16, 1, d['S'], d['H'], d['dh'], 0.0, 0, 0, 0, 16, None)",
+    }
+    made = {"attention": "t.attn(**kw)", "linear_attention": "t.lin(**kw)", "step": "kw", "mhsa": "{**dict(S=200, H=2, dh=16), **kw}"}
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = (f"import sys; sys.path[:0] = [{os.path.dirname(here) + '/news-recommendation_amd'!r}, {here!r}]\nfrom newsrec_hip import _lib\n"
+            f"import test_sequence_ops_cpu as t\nkw = {kw!r}\nd = {made[what]}\nL = _lib.load()\nprint(*({calls[what]}))")
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0, (got.returncode, got.stderr[-500:])
+    assert set(got.stdout.split()) == {"2"}, got.stdout      # NR_ERR_UNSUPPORTED, and no workspace
