@@ -1,4 +1,5 @@
-"""what ops.attention, ops.linear_attention and ops.linear_attention_step refuse before any device call"""
+"""what ops.attention, ops.linear_attention and ops.linear_attention_step refuse before any device call, and the arithmetic behind the bounds
+of test_gpu_sequence_edges.py"""
 import math
 import os
 import subprocess
@@ -8,6 +9,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import fp32_oracle
 from newsrec_hip import ops
 from newsrec_hip._lib import NewsrecError
 
@@ -83,3 +85,53 @@ def test_sizes_past_the_kernels_integers_are_refused(what, kw):
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert got.returncode == 0, (got.returncode, got.stderr[-500:])
     assert set(got.stdout.split()) == {"2"}, got.stdout      # NR_ERR_UNSUPPORTED, and no workspace
+
+
+# ----------------------------------------------------------------------------- fp32 numbers as bf16 parts
+def parts(t, n):
+    """what the kernels make of an fp32 number: n bf16 parts, each cut off after 8 bits"""
+    rest, out = t.float().clone(), []
+    for _ in range(n):
+        cut = (rest.contiguous().view(torch.int32) & -65536).view(torch.float32)
+        out.append(cut.double())
+        rest = rest - cut
+    return out
+
+
+def split_product(a, b, n=3):
+    """a @ b (64-bit sums) as the kernels form it: the partial products of the parts whose numbers add up to less than n"""
+    x, y = parts(a, n), parts(b, n)
+    return sum(x[i] @ y[j] for i in range(n) for j in range(n - i))
+
+
+def test_what_three_parts_leave_out():
+    """below 2^-21 of a product, one-sided, near 2^-24.5 on average"""
+    a = torch.tensor([[1 + 2.0 ** -7 - 2.0 ** -23]])
+    left = float((a.double() ** 2 - split_product(a, a)) / a.double() ** 2)
+    assert 2.0 ** -21.2 < left < 2.0 ** -21                       # near the worst case
+    g = torch.Generator().manual_seed(0)
+    x, y = (torch.randn(100000, 1, 1, generator=g) for _ in range(2))
+    exact = x.double() @ y.double()
+    left = (exact - split_product(x, y)) / exact
+    assert bool((left >= 0).all()) and float(left.max()) < 2.0 ** -21
+    assert 2.0 ** -25 < float(left.mean()) < 2.0 ** -24
+
+
+SITES = ("qk", "pv", "dov", "pdo", "dsk", "dsq")
+
+
+@pytest.mark.parametrize("Sq", [3, 40])
+@pytest.mark.parametrize("d", [1, 2])
+def test_the_fp32_bounds_see_a_lost_part(d, Sq):
+    """operands of three parts stay within fp32_oracle's bounds in every product; cut to two in any one of them they do not"""
+    seen = set()
+    for spread in (1.0, 2.0 ** -6):
+        q, k, v, do = fp32_oracle.small_problem(spread, d, Sq, "cpu")
+        want = fp32_oracle.reference(q, k, v, do)
+        off = lambda got: max(float(((got[n][0] - want[n][0]).abs() / want[n][1].clamp_min(1e-300)).max()) for n in want)    # noqa: E731
+        assert off(fp32_oracle.reference(q, k, v, do, lambda site, a, b: split_product(a, b))) < 0.5
+        for site in SITES:
+            lost = lambda at, a, b: split_product(a, b, 2 if at == site else 3)           # noqa: E731
+            if off(fp32_oracle.reference(q, k, v, do, lost)) > 1.5:
+                seen.add(site)
+    assert seen == set(SITES), seen
