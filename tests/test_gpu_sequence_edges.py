@@ -101,3 +101,117 @@ def test_fp32_meets_the_bars_of_the_short_kernels(ops, size, causal):
     want = attention_oracle.reference(q, k, v, None, causal, do=do)
     for name, t in zip(("o", "dq", "dk", "dv"), A.run(ops, q, k, v, do, causal=causal)):
         assert relerr(t, want[name][0]) < (1e-5 if name == "o" else 2e-5), name
+
+
+def steepest(f, noise, x, grad, h):
+    """the derivative of f along its own gradient at x: (from the gradient, from central differences over h and h / 2 with the h^2 term
+    taken out, how far the two may be apart).  noise: how far one value of f may be off"""
+    r = grad / grad.double().norm().item()
+    with torch.no_grad():
+        far, near = ((f(x + s * r) - f(x - s * r)) / (2 * s) for s in (h, h / 2))
+    slope = float((grad.double() * r.double()).sum())
+    return slope, (4 * near - far) / 3, abs(near - far) / 3 + 3 * noise / h
+
+
+@pytest.mark.parametrize("Sq", [3, 37], ids=["few rows", "rows"])
+def test_attention_falls_as_its_gradients_say(ops, Sq):
+    """central differences of the kernel's own forward along each gradient, where the slope is largest: a gradient 5 % too long or too
+    short, or turned by as much as that takes off its length, is outside the tolerance"""
+    size = (1, Sq, 9, 2, 1, 8)
+    ts = A.make(44, *size, F32)
+    got = A.run(ops, *ts)
+    noise = float((attention_oracle.reference(*ts[:3])["o"][1] * ts[3].double().abs()).sum())
+    for i, name in enumerate("qkv"):
+        def f(x, i=i):
+            return float((ops.attention(*ts[:i], x, *ts[i + 1:3]).double() * ts[3].double()).sum())
+        slope, best, tol = steepest(f, noise, ts[i], got[1 + i], 0.25)
+        assert tol < 0.05 * slope, (name, slope, tol)
+        assert abs(best - slope) <= tol, (name, slope, best, tol)
+
+
+@pytest.mark.parametrize("S", [9, 50])
+def test_linear_attention_falls_as_its_gradients_say(ops, S):
+    """the same of linear attention, whose outputs are linear in each operand: no h^2 term, so a long step"""
+    t, a = L.make(45, 1, S, 2, 8, 6, F32), L.decays(2)
+    got = L.run(ops, t, a)
+    ref = L.reference(t["q"], t["k"], t["v"], a, None, t["state"])
+    noise = float((ref["o"][1] * t["do"].double().abs()).sum() + (ref["last"][1] * t["dlast"].double().abs()).sum())
+    for n in ("q", "k", "v", "state"):
+        def f(x, n=n):
+            now = {**t, n: x}
+            o, last = ops.linear_attention(now["q"], now["k"], now["v"], a, state=now["state"])
+            return float((o.double() * t["do"].double()).sum() + (last.double() * t["dlast"].double()).sum())
+        # (at twice the step the sums over absolute values may be a few times larger than at t itself)
+        slope, best, tol = steepest(f, 4 * noise, t[n], got["d" + n], 4.0)
+        assert tol < 0.05 * slope, (n, slope, tol)
+        assert abs(best - slope) <= tol, (n, slope, best, tol)
+
+
+def subsets(names):
+    return [[n for i, n in enumerate(names) if b >> i & 1] for b in range(1, 2 ** len(names) - 1)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_gradients_of_some_inputs(ops, dtype):
+    """whichever inputs ask for a gradient, each gets the one it gets when all ask.  (Linear attention on bf16 tensors carries its state
+    in three bf16 parts where the state's own gradient is asked for and in two where it is not: each compared with its like.)"""
+    t = dict(zip(("q", "k", "v", "do"), A.make(46, 2, 70, 75, 4, 2, 64, dtype)))
+    m = A.make_mask("prefix", 3, 2, 75)
+
+    def grads(names):
+        x = {n: t[n].detach().requires_grad_(n in names) for n in "qkv"}
+        return dict(zip(names, torch.autograd.grad(ops.attention(*x.values(), key_mask=m), [x[n] for n in names], t["do"])))
+
+    want = grads("qkv")
+    for names in subsets("qkv"):
+        for n, g in grads(names).items():
+            assert torch.equal(g, want[n]), (names, n)
+    t, a = L.make(47, 2, 90, 2, 32, 48, dtype), L.decays(2)
+    lens = torch.tensor([90, 41], device="cuda")
+
+    def grads(names):                                                                      # noqa: F811
+        x = {n: t[n].detach().requires_grad_(n in names) for n in ("q", "k", "v", "state")}
+        out = ops.linear_attention(x["q"], x["k"], x["v"], a, lens=lens, state=x["state"])
+        return dict(zip(names, torch.autograd.grad(out, [x[n] for n in names], (t["do"], t["dlast"]))))
+
+    every = {True: grads(["q", "k", "v", "state"]), False: grads(["q", "k", "v"])}
+    for names in subsets(["q", "k", "v", "state"]):
+        for n, g in grads(names).items():
+            assert torch.equal(g, every["state" in names][n]), (names, n)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("mask", ["prefix", "holes"])
+@pytest.mark.parametrize("size", [(2, 40, 71, 2, 2, 25), (2, 130, 133, 4, 2, 64), (2, 3, 701, 2, 1, 64), (2, 50, 50, 2, 2, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_dropout_beside_a_mask(ops, size, mask, causal, dtype):
+    """rows whose first probability is not the first of four numbers of the stream (Sk % 4 != 0), keys that are not there between them"""
+    N, Sq, Sk, H, G, d = size
+    q, k, v, do = A.make(48, *size, dtype)
+    m = A.make_mask(mask, 5, N, Sk)
+    keep = keep_mask((N, H, Sq, Sk), 0.1, 78, 5)
+    want = attention_oracle.reference(q, k, v, m, causal, do=do, keep=keep, p_drop=0.1)
+    for name, t in zip(("o", "dq", "dk", "dv"), A.run(ops, q, k, v, do, key_mask=m, causal=causal, p_drop=0.1, seed=78, site=5)):
+        check(name, t, want[name])
+
+
+@pytest.mark.parametrize("dh", [33, 40, 64])
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("hf", [False, True], ids=["additive", "excluded"])
+def test_mhsa_whose_forward_alone_is_long(ops, dh, p, hf):
+    """128 positions of more than 32 columns: too much LDS for the short forward, so the key-tiled one runs and leaves its statistics to the
+    short kernels' backward.  Bars of test_mhsa_past_the_short_kernels"""
+    N, S, H = 3, 128, 2
+    g = torch.Generator().manual_seed(dh)
+    qkv, dctx = torch.randn(N * S, 3 * H * dh, generator=g), torch.randn(N * S, H * dh, generator=g)
+    mask = (torch.arange(S)[None] < torch.tensor([[S], [70], [0 if hf else 1]])).long()
+    keep = keep_mask((N, H, S, S), p, 99, 3) if p else None
+    x = qkv.double().requires_grad_(True)
+    ref = A._mhsa_ref(x, mask, N, S, H, dh, keep, p, not hf)
+    ref.backward(dctx.double())
+    leaf = qkv.cuda().requires_grad_(True)
+    ctx = ops.mhsa(leaf, mask.cuda(), N, S, H, dh, p, 99, 3, hf_mask=hf)
+    (dqkv,) = torch.autograd.grad(ctx, (leaf,), dctx.cuda())
+    assert relerr(ctx, ref) < 1e-5
+    assert relerr(dqkv, x.grad) < 2e-5
