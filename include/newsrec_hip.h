@@ -143,7 +143,9 @@ int nr_add_layernorm_bwd_noalloc_f32(const float* dy, const float* s, const floa
  * mask_mode 1: masked keys are excluded and a sequence without any valid key gets zero probabilities — what
  *   HF BertModel computes under torch SDPA for AllBertNewsEncoder (encoder.py:74; transformers 5.15 / torch 2.10).
  * Any S (up to 2^30); head dims up to 128.  Sequences of S <= 128 run on kernels that hold a whole head at once, longer ones (and the head dims
- * those kernels do not take) on the key-tiled kernels of nr_attention_fwd / _bwd below, which S has no bound for. */
+ * those kernels do not take) on the key-tiled kernels of nr_attention_fwd / _bwd below, which S has no bound for.  Without a workspace
+ * argument they are not split along S: with fewer than 256 blocks of 128 rows (N * H * S / 128) of more than 512 positions,
+ * nr_attention_* on the same operands is up to twice as fast. */
 int nr_mhsa_fwd_f32(const float* qkv, const int64_t* mask, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* ctx, float* row_max, float* row_sum, void* stream);
 int nr_mhsa_bwd_f32(const float* qkv, const int64_t* mask, const float* ctx, const float* dctx, const float* row_max, const float* row_sum, int64_t N, int64_t S, int64_t H, int64_t dh, float p_drop, uint64_t seed, uint32_t site, int mask_mode, float* dqkv, void* stream);
 /* The same core on bf16 tensors (raw 16-bit storage; S <= 32, head dim <= 64): what the bf16 build of AllBertNewsEncoder's

@@ -342,7 +342,9 @@ constexpr size_t MHSA_LDS_MAX = 160 * 1024;    // one workgroup may take the CU'
 static int pick_dhp(int dh) { return dh <= 32 ? 32 : (dh <= 64 ? 64 : (dh <= 128 ? 128 : 0)); }
 
 // sequences past 128 positions, and head dims past what the kernels above hold in LDS: the key-tiled kernels of
-// attention_long*.hip on the q | k | v blocks of the packed rows, with this layer's additive mask
+// attention_long*.hip on the q | k | v blocks of the packed rows, with this layer's additive mask.  The entry points have no workspace
+// argument, so the long axis is never split here, and a few long sequences leave CUs idle: one of 1024, 12 heads of 64: forward 67 us, with
+// the backward 268 (nr_attention_*, split: 39 and 152); of 2048: 126 and 513 (109 and 459); one or four of 512, four of 2048: the same.
 static AttnProblem long_problem(const float* qkv, const int64_t* mask, int64_t N, int S, int H, int dh, const DropoutCfg& dc) {
     AttnProblem p;
     const int64_t A = (int64_t)H * dh;

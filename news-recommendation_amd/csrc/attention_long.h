@@ -1,4 +1,4 @@
-// internal interface of the attention kernels without a bound on the sequence length (attention_long.hip, attention_long_bwd.hip)
+// internal interface of the attention kernels without a bound on the sequence length (attention_long*.hip)
 #pragma once
 #include "common.h"
 #include "rowops.h"

@@ -21,7 +21,12 @@ static bool all_aligned(const AttnProblem& p) {
     const size_t e = p.bf16 ? 2 : 4;
     return aligned16(p.q, p.sq, p.dh, e, 128) && aligned16(p.k, p.sk, p.dh, e, 128) && aligned16(p.v, p.sv, p.dh, e, 128);
 }
-// workgroups that do not reach every CU split `length` further, to about two per CU and down to 256 of it each
+// Workgroups that do not reach every CU split `length` further, to about two per CU and down to 256 of it each.  Both sides, us of device
+// time, forward / forward and backward: 15 rows over 20011 keys, 4 x 4 key heads of 64, bf16: split 21 / 123, whole 139 / 353; one sequence of 2048,
+// 12 heads of 64: bf16 36.5 / 135 and 36 / 155, fp32 104 / 437 and 115 / 478; one of 1000, 8 heads of 128, fp32: 58 / 227 and 112 / 483;
+// single queries over 1000 keys, 8 x 12 heads of 64, bf16: 12 / 44 either way.  Other aims: one workgroup per CU 34.7 / 135 (bf16) and 94 /
+// 384 (fp32) on the sequence of 2048, but four 40 / 157 and 102 / 416.  Down to 128: fp32 wins where few heads are short (one sequence of 512,
+// 12 heads of 64: 35 / 135 whole, 20 / 76 in four), bf16 loses where they are more (4 x 512: 12.7 / 53 whole, 19 / 74).
 static Split split_axis(int64_t blocks, int length, int unit) {
     Split s{1, length};
     if (blocks <= 0 || blocks >= 256 || length <= 512) return s;
@@ -37,6 +42,9 @@ struct FwdPlan { int wk, nblk, head_blocks; Split sp; size_t ws; };
 static FwdPlan plan_fwd(const AttnProblem& p) {
     FwdPlan f;
     const int64_t R = (int64_t)(p.H / p.G) * p.Sq;
+    // Few rows share the waves.  33 to 64 of them could in two blocks: better where they have many keys or few heads (64 x 1000 keys, 32 x 4
+    // heads of 64, bf16: 18 us as here, 13 shared; 36 x 200, fp32: 14 and 10), worse where there are blocks enough (50 x 50, 64 x 12 heads of
+    // 64, bf16: 7.5 and 17 us; 33 x 300, 32 x 12: 11 and 15).
     f.wk = R <= 32 ? 4 : 1;
     f.head_blocks = f.wk == 1 ? head_blocks(p, 128) : 0;
     f.nblk = f.head_blocks ? p.H / p.G * f.head_blocks : cdiv(R, 32 * (4 / f.wk));

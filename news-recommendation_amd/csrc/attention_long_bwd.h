@@ -15,8 +15,15 @@
 // Measured (MI355X).  4001 x 4001 causal, 16 heads (4 of them with keys) of 128, bf16: dQ 160 us (600 TFLOP/s of its three products),
 // dK / dV 222 us (580 of its four), 19 us to join the splits.  dK / dV holds K and V fragments and both sums, 256 registers at 128
 // columns: one wave per SIMD, so a tile's LDS reads and exponentials are hidden only by its own products.  16 x 512 ragged, 12 heads
-// of 64, bf16: dQ 34 us, dK / dV 41 us (three waves per SIMD); fp32 histories of 200, 12 heads of 25: 42 and 52 us, bound by the
-// latency of a block's few tiles.
+// of 64, bf16: dQ 34 us, dK / dV 41 us (three waves per SIMD; 52 on average in one run of two); fp32 histories of 200, 12 heads of 25: 42
+// and 52 us, bound by the latency of a block's few tiles.  Dropout of 0.1: the same texts dQ 78 us, dK / dV 209 (a call of the generator
+// per element, of whose four numbers one is used: a lane's elements are rows of one key); the histories 63 and 94; 16 x 512, 12 heads of
+// 64 in fp32: 143 and 293.
+//
+// Registers that do not fit and go to scratch memory, per lane (in brackets where addresses are unaligned): dK / dV, bf16, 64 columns 9
+// (22), fp32, 64 columns 10 (20), 128 columns 61 (78); dQ, fp32, 128 columns and few rows 0 (285), 64 columns 0 (28), bf16, 128 columns 0
+// (36), its one-tile form 34 (116).  With dropout: dK / dV, bf16, 32 columns 29 (60), 64 columns 128 (265), fp32, 64 columns 74 (86), 128
+// columns 98 (115); dQ, fp32, 64 columns 27 (40), 128 columns and few rows 18 (300), bf16, 128 columns 18 (61), one-tile form 62 (187).
 #pragma once
 #include "attention_long_dev.h"
 

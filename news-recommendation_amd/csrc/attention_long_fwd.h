@@ -19,10 +19,16 @@
 //
 // Measured (MI355X).  Long rows are bound by issue: per 64 keys and 32 rows a wave has 2 * 64 * 32 * 2 * dh operations for the matrix
 // pipe beside 2048 exponentials with their maximum and sum on the vector pipe.  8192 x 8192 causal, 16 heads (4 of them with keys) of
-// 128, bf16: 309 us, 890 TFLOP/s, where a large matrix product of the library reaches 1363; heads of 64 without causal order: 700
-// TFLOP/s (the exponentials weigh twice as much); fp32, 4096 x 64: 185 TFLOP/s (105 on the fp32 matrix instruction).  Short ones are
-// bound by the latency of a block's few tiles and the last round of workgroups: 32 x 512 ragged, 12 heads of 64, bf16: 38 us, 2.6 TB/s
-// and 410 TFLOP/s; 32 fp32 histories of 200, 12 heads of 25: 24 us.  5 rows over 20011 keys in splits: 19 us + 4 for the join, 4.3 TB/s of keys.
+// 128, bf16: 309 - 323 us a pass by card, 850 - 890 TFLOP/s, where a large matrix product of the library reaches 1363 (a launch on its
+// own under the profiler, at a lower clock: 352 - 372); heads of 64 without causal order: 700 TFLOP/s (the exponentials weigh twice as
+// much); fp32, 4096 x 64: 185 TFLOP/s (105 on the fp32 matrix instruction).  Short ones are bound by the latency of a block's few tiles
+// and the last round of workgroups: 32 x 512 ragged, 12 heads of 64, bf16: 36 - 37 us a pass (39.5 - 42 on its own), 2.8 TB/s and 430
+// TFLOP/s; 32 fp32 histories of 200, 12 heads of 25: 24 us (25.5 - 27).  5 rows over 20011 keys in splits: 19 us + 4 for the join, 4.3
+// TB/s of keys.  Dropout of 0.1: 16 x 512 ragged, 12 heads of 64, bf16: 24 -> 67 us, 85 where Sk is no multiple of 4 (keep4 then calls
+// the generator twice); the fp32 histories 27 -> 53: the generator takes the difference.
+//
+// Registers that do not fit and go to scratch memory: 128 columns in fp32 with few rows and unaligned addresses 158 per lane; 128 columns
+// in bf16, unaligned, 7 (45 with dropout).  The others hold all of theirs.
 #pragma once
 #include "attention_long_dev.h"
 

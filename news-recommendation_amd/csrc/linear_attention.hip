@@ -28,7 +28,9 @@
 // one wave for everything took about 7300 cycles per 64 tokens (scores and output 1180 and state 1330 per chunk, stores 400, LDS 510,
 // loads 430), which the pairs of waves divide.  32 sequences up to 1000 tokens, 12 heads: forward 60 us (73 with one wave), backward 100
 // (111).  2 x 16384 tokens, 12 heads, in 32 segments: segment sums 26 us, scan 9 us, output 45 us: 2.5 TB/s in all, 3.8 with the
-// second read of k and v.  128 x 1000 tokens, 12 heads: forward 201 us, 3.9 TB/s.
+// second read of k and v.  128 x 1000 tokens, 12 heads: forward 201 us, 3.9 TB/s.  One wave for everything, the same 32 sequences: bf16,
+// 128 wide: forward 147 us, backward 320; fp32, 64 wide (on the fp32 matrix instruction): 201 and 265; 128 wide a pass of both 1250.
+// lin_pair_kernel at unaligned 64 x 32 widths puts 17 registers per lane into scratch memory, lin_out_kernel at unaligned 128 x 32 in bf16 25.
 #include "linear_attention.h"
 #include "attention_long_dev.h"
 #include <algorithm>
@@ -531,9 +533,11 @@ __global__ __launch_bounds__(256) void lin_step_kernel(const T* __restrict__ q, 
 
 // ---------------------------------------------------------------- host
 // heads * sequences that leave the chip part empty are cut into segments, down to 256 tokens each, at least three of them, and only past
-// 1024 tokens: the extra pass reads y and z again, and a scan follows it (16 x 12 ragged heads of 1000 x 64: 35 us whole, 46 us in
-// three; 2 x 12 of 16384: 69 us in 32).  Aimed at as many workgroups as the chip holds at once: three per CU of the pair kernel (512:
-// 73 us, 1024: 83), four of the other.
+// 1024 tokens: the extra pass reads y and z again, and a scan follows it.  Sequences of 1000 tokens of 12 heads, whole and in three, us of
+// device time, forward / forward and backward: 16 of them, bf16, 64 wide: 34 / 87 and 48 / 101; 4 of them: 33 / 64 and 31 / 71; one: 33 / 63
+// and 29 / 58.  Where one wave does everything whole sequences lose there: one, bf16, 128 wide: 78 / 148 and 54 / 114; one, fp32, 25 wide:
+// 135 / 267 and 80 / 160 (in eight of 128 tokens: 46 / 95).  2 x 12 of 16384, bf16, in 32: 80 us.  Aimed at as many workgroups as the chip holds
+// at once: three per CU of the pair kernel (512 workgroups: 73 us, 768: 69, 1024: 83), four of the other.
 static void cut(Args& a, bool bf16) {
     const int64_t blocks = a.jobs * a.N * a.H, aim = bf16 && a.job[0].da <= 64 && a.job[0].db <= 64 ? 768 : 1024;
     a.G = 1; a.per = (a.S + UNIT - 1) / UNIT * UNIT;
