@@ -500,6 +500,8 @@ def _no_tangent(what, *tensors):
 
 def _scale(what, scale):
     """a factor that crosses the C boundary in fp32"""
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise NewsrecError(f"{what}: scale is a number here, it has no gradient (detach it, or scale q)")
     scale = float(scale)
     if not abs(scale) <= _FP32_MAX:
         raise NewsrecError(f"{what}: scale {scale} is not a number within fp32's range")

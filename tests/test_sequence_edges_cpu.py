@@ -61,6 +61,17 @@ def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
             ops.attention(x, x, x, scale=s)
 
 
+def test_a_scale_that_expects_a_gradient_is_refused():
+    """float() of it would leave the gradient out"""
+    x, one, scale = torch.ones(1, 3, 2, 4), torch.ones(1, 2, 4), torch.tensor(0.5, requires_grad=True)
+    for call in (lambda s: ops.attention(x, x, x, scale=s), lambda s: ops.linear_attention(x, x, x, torch.zeros(2), scale=s),
+                 lambda s: ops.linear_attention_step(one, one, one, torch.zeros(2), torch.zeros(1, 2, 4, 4), scale=s)):
+        with pytest.raises(NewsrecError, match="scale.*no gradient"):
+            call(scale)
+        with pytest.raises(NewsrecError, match="ROCm"):
+            call(scale.detach())
+
+
 # sizes whose products or fp32-sized integers wrap: each in a process of its own, since what this refuses used to end it
 HUGE = [("attention", dict(H=1 << 32, G=1 << 32, Sq=1)), ("attention", dict(H=1 << 62, G=1, Sq=8)), ("attention", dict(N=1 << 62, H=4, G=4)),
         ("attention", dict(N=1 << 40, H=1 << 24, G=1 << 24, Sq=1)), ("linear_attention", dict(N=1 << 62)), ("linear_attention", dict(N=1 << 31, H=4)),
