@@ -215,3 +215,146 @@ def test_mhsa_whose_forward_alone_is_long(ops, dh, p, hf):
     (dqkv,) = torch.autograd.grad(ctx, (leaf,), dctx.cuda())
     assert relerr(ctx, ref) < 1e-5
     assert relerr(dqkv, x.grad) < 2e-5
+
+
+# ----------------------------------------------------------------------------- calls that the documentation allows
+@pytest.mark.parametrize("S,step", [(600, 1 << 22), (150, 1 << 24)], ids=["32-bit tiles", "64-bit tiles"])
+def test_gradients_of_rows_far_apart(ops, S, step):
+    """operands whose offsets pass 2^31 elements, with tiles that a 32-bit offset still spans and with wider ones: the same bits as from
+    dense copies, forward and backward, and from linear attention with a length that ends inside"""
+    room = torch.empty((S - 1) * step + 4096, dtype=BF16, device="cuda")
+    dense = A.make(50, 1, S, S, 2, 2, 64, BF16)
+    far = []
+    for i, t in enumerate(dense[:3]):
+        far.append(room.as_strided((1, S, 2, 64), (0, step, 64, 1), 512 * i))
+        far[-1].copy_(t)
+    m = A.make_mask("holes", 6, 1, S)
+    for a, b in zip(A.run(ops, *far, dense[3], key_mask=m, causal=True), A.run(ops, *dense, key_mask=m, causal=True)):
+        assert torch.equal(a, b)
+    lens = torch.tensor([S - 7], device="cuda")
+    got = []
+    for q, k, v in (far, dense[:3]):
+        t = dict(q=q, k=k, v=v, do=dense[3], state=None, dlast=None)
+        got.append(L.run(ops, t, L.decays(2), lens, carried=False, both=False))
+    for n in got[0]:
+        assert torch.equal(got[0][n], got[1][n]), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(2, 5, 3001, 6, 2, 25), (1, 40, 2000, 2, 2, 33), (1, 700, 700, 4, 2, 128), (3, 70, 75, 2, 2, 64)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_nothing_is_read_that_the_call_did_not_write(ops, size, dtype):
+    """memory that the allocator hands out again holds NaN: workspaces, statistics and outputs are written before they are read"""
+    q, k, v, do = A.make(51, *size, dtype)
+    m = A.make_mask("prefix", 7, size[0], size[2])
+    m[0] = 0
+    want = A.run(ops, q, k, v, do, key_mask=m, causal=True, p_drop=0.1, seed=3)
+    t, a = L.make(52, 1, size[2], 2, min(size[5], 64), 40, dtype), L.decays(2)
+    lens = torch.tensor([size[2] // 2], device="cuda")
+    rec = L.run(ops, t, a, lens)
+    for _ in range(2):
+        waste = [torch.full((1 << p,), math.nan, device="cuda") for p in range(6, 24) for _ in range(3)]
+        del waste
+        for x, y in zip(A.run(ops, q, k, v, do, key_mask=m, causal=True, p_drop=0.1, seed=3), want):
+            assert torch.equal(x, y)
+        waste = [torch.full((1 << p,), math.nan, device="cuda") for p in range(6, 24) for _ in range(3)]
+        del waste
+        for n, x in L.run(ops, t, a, lens).items():
+            assert torch.equal(x, rec[n]), n
+
+
+@pytest.mark.parametrize("S,dh", [(200, 25), (128, 64)])
+def test_layer_core_captured_and_replayed(ops, S, dh):
+    """ops.mhsa past the short kernels, forward and backward with dropout in one graph, replayed on new inputs"""
+    N, H = 2, 4
+    A_ = H * dh
+    g = torch.Generator(device="cuda").manual_seed(53)
+    draw = lambda: (torch.randn(N * S, 3 * A_, generator=g, device="cuda"), torch.randn(N * S, A_, generator=g, device="cuda"),      # noqa: E731
+                    (torch.rand(N, S, generator=g, device="cuda") < 0.7).long())
+    held = draw()
+
+    def both(qkv, dctx, mask):
+        leaf = qkv.detach().requires_grad_(True)
+        ctx = ops.mhsa(leaf, mask, N, S, H, dh, 0.1, 7, 1)
+        return (ctx.detach(),) + torch.autograd.grad(ctx, (leaf,), dctx)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(*held)
+    for _ in range(3):
+        new = draw()
+        for x, y in zip(held, new):
+            x.copy_(y)
+        want = both(*new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_one_tensor_for_everything_and_saved_elsewhere(ops, dtype):
+    """q, k and v one leaf, whose gradient is the sum of the three; two backward passes of one graph; and the saved tensors kept on the host"""
+    x, _, _, do = A.make(54, 2, 90, 90, 4, 4, 40, dtype)
+    parts_ = A.run(ops, x, x, x, do)
+    leaf = x.detach().requires_grad_(True)
+    o = ops.attention(leaf, leaf, leaf)
+    (first,) = torch.autograd.grad(o, leaf, do, retain_graph=True)
+    (again,) = torch.autograd.grad(o, leaf, do)
+    assert torch.equal(first, again)
+    # (autograd adds the three in some order of its own, each addition rounded to the type: two half steps of the absolute values)
+    exact = sum(t.double() for t in parts_[1:])
+    size = sum(t.double().abs() for t in parts_[1:])
+    assert bool(((first.double() - exact).abs() <= 2.02 * torch.finfo(dtype).eps / 2 * size).all())
+    with torch.autograd.graph.save_on_cpu():
+        o = ops.attention(leaf, leaf, leaf)
+        r, last = ops.linear_attention(leaf, leaf.expand(2, 90, 4, 40), leaf, L.decays(4))
+    assert torch.equal(torch.autograd.grad(o, leaf, do)[0], first)
+    assert bool(torch.isfinite(torch.autograd.grad(r, leaf, do)[0].float()).all())
+
+
+def test_many_sequences(ops):
+    """more workgroups than a 16-bit grid axis, sequences of a few tokens; the step over as many heads"""
+    N, H, d = 40000, 2, 8
+    q, k, v, do = A.make(55, N, 1, 3, H, H, d, F32)
+    m = A.make_mask("prefix", 8, N, 3)
+    want = attention_oracle.reference(q, k, v, m, do=do)
+    for name, t in zip(("o", "dq", "dk", "dv"), A.run(ops, q, k, v, do, key_mask=m)):
+        check(name, t, want[name])
+    a, state = L.decays(H), torch.zeros(N, H, d, d, device="cuda")
+    outs = [ops.linear_attention_step(k[:, i], k[:, i], v[:, i], a, state) for i in range(3)]
+    o, last = ops.linear_attention(k, k, v, a)
+    # both are within fp32's few roundings of the definition: dots of 8, sums of 3, a power's 2^-22
+    size = (k.double().abs().sum(1).amax(-1) ** 2 * 3).amax() * v.abs().max()
+    assert float((torch.stack(outs, 1) - o).abs().max()) <= 2.0 ** -20 * float(size)
+    assert float((state - last).abs().max()) <= 2.0 ** -20 * float(size)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_a_long_record(ops, dtype):
+    """100 003 tokens of one head in many segments, against the same record walked in four carried pieces and its last 300 tokens against the
+    definition with the state that stood before them"""
+    S, d = 100003, 32
+    t, a = L.make(56, 1, S, 1, d, d, dtype), torch.tensor([-0.01], device="cuda")
+    o, last = ops.linear_attention(t["q"], t["k"], t["v"], a)
+    state, outs = None, []
+    cuts = [0, 30000, 30001, 99703, S]
+    for lo, hi in zip(cuts, cuts[1:]):
+        before = state
+        p, state = ops.linear_attention(t["q"][:, lo:hi], t["k"][:, lo:hi], t["v"][:, lo:hi], a, state=state)
+        outs.append(p)
+    tail = {n: t[n][:, -300:] for n in ("q", "k", "v")}
+    want = L.reference(tail["q"], tail["k"], tail["v"], a, None, before)
+    check("o of the pieces", outs[-1], want["o"])
+    # the whole walk's state before the tail is another sum of the same tokens: memories of 100 tokens weigh 2^-150 after 10 400, so
+    # both are within the bound of a record of that length (e = 2^-24 * 10 400 * 9 / 8 of the absolute values, u^3 of them for bf16)
+    mem = L.reference(t["q"][:, -10400:], t["k"][:, -10400:], t["v"][:, -10400:], a)
+    for name, x in (("o", o[:, -300:]), ("last", last)):
+        value, bound = (y[:, -300:] if name == "o" else y for y in mem[name])
+        check(name + " of the whole", x, (value, bound + 1e-30))
+    check("last of the pieces", state, mem["last"])
