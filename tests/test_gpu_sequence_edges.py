@@ -358,3 +358,34 @@ def test_a_long_record(ops, dtype):
         value, bound = (y[:, -300:] if name == "o" else y for y in mem[name])
         check(name + " of the whole", x, (value, bound + 1e-30))
     check("last of the pieces", state, mem["last"])
+
+
+@pytest.mark.parametrize("T", [160, 512])
+def test_bert_past_128_positions(ops, T):
+    """HipBertModel over long texts, one of them a single token, states and every gradient against the CPU oracle's.  Bars of
+    test_layer_over_long_histories"""
+    from models.modules.encoder import HipBertModel
+    from oracle import twotower_oracle as O
+    torch.manual_seed(T)
+    plm = HipBertModel(dict(vocab_size=60, hidden_size=64, num_attention_heads=2, num_hidden_layers=2, intermediate_size=256,
+                            max_position_embeddings=512, type_vocab_size=2, layer_norm_eps=1e-12, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0,
+                            initializer_range=0.2))
+    ids, lens = torch.randint(1, 60, (3, T)), torch.tensor([T, 1, T - 31])
+    mask = (torch.arange(T)[None] < lens[:, None]).long()
+    P = {"newsEncoder.plm." + k: v.detach().clone().double().requires_grad_(True) for k, v in plm.state_dict().items()}
+    ref = O.bert_news_encoder(P, ids, mask, 2)[0]
+    dy = torch.randn(3, T, 64)
+    ref.backward(dy.double())
+    plm = plm.cuda().train()
+    out = plm(ids.cuda(), mask.cuda())
+    out.backward(dy.cuda())
+    assert relerr(out, ref) < 1e-5
+    for n, p in plm.named_parameters():
+        r = P["newsEncoder.plm." + n].grad
+        if n.endswith("key.bias"):
+            # exactly zero: a constant added to every key moves a row's scores alike.  What is left is the error of sum_j dK_j; that of the
+            # weight's gradient, sum_j dK_j x_j, is of the same rows times x_j of mean square 1 (a LayerNorm's), so its size measures both.
+            assert r.abs().max().item() < 1e-10
+            assert p.grad.abs().max().item() <= 5e-5 * P["newsEncoder.plm." + n[:-4] + "weight"].grad.abs().max().item() + 1e-6, n
+            continue
+        assert (p.grad.cpu().double() - r).abs().max().item() <= 5e-5 * r.abs().max().item() + 1e-6, n
